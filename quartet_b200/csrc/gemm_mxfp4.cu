@@ -105,25 +105,6 @@ __device__ __forceinline__ uint32_t make_idesc(int n, uint32_t sf_id) {
     return d;
 }
 
-// Bounded wait on wall-clock time (2 s), for the pipeline barriers.
-__device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, int32_t who, volatile int* dead) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*dead) return false;
-    uint64_t t0 = 0;
-    for (uint32_t i = 0;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 1023u) == 1023u) {
-            uint64_t now;
-            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-            if (t0 == 0) t0 = now;
-            if (now - t0 > 2000000000ull || *dead) break;
-        }
-    }
-    atomicOr(&g_status, who | 0x100);
-    *dead = 1;
-    return false;
-}
-
 // Epilogue of one 32-row x 32-column block held as one accumulator row per thread: scale, optional
 // mask + un-rotation (the 32 columns are exactly one Hadamard group), convert, stage 32 rows x 64
 // bytes in swizzled shared memory and hand them to TMA -- one store of 32 rows x 64 bytes for bf16, two
@@ -422,59 +403,6 @@ struct Gemm2Cfg {
     static_assert(B_BYTES % 1024 == 0, "operand stages stay 1024-byte aligned");
 };
 
-// One lane of a fully converged warp (elect.sync): the issuing warp runs its loop on all 32 lanes so
-// that ring indices, descriptors and addresses stay warp-uniform, and only the tcgen05 instructions
-// themselves are predicated on the elected lane.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred = 0;
-    asm volatile(
-        "{\n\t.reg .b32 rx;\n\t.reg .pred px;\n\t"
-        "elect.sync rx|px, 0xFFFFFFFF;\n\t"
-        "selp.u32 %0, 1, 0, px;\n\t}"
-        : "=r"(pred));
-    return pred != 0;
-}
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t mapa_u32(uint32_t saddr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    // default semantics (as the pipelines of CUTLASS use for consumer -> producer signalling across
-    // CTAs); an explicit .release.cluster here costs ~1500 cycles per arrive
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish2() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// arrive on a barrier (given by its shared::cluster address) once all MMAs issued so far are done
-__device__ __forceinline__ void tc_commit2(uint32_t cluster_addr) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr)
-                 : "memory");
-}
-// the same, arriving on the barrier at this shared-memory offset in BOTH CTAs of the pair (one
-// instruction instead of two commits; only the completion signal is multicast, no data copy)
-__device__ __forceinline__ void tc_commit2_pair(uint32_t own_addr) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                     own_addr),
-                 "h"((uint16_t)3)
-                 : "memory");
-}
 __device__ __forceinline__ void tc_mma2_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                              uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
     asm volatile(
@@ -494,18 +422,6 @@ __device__ __forceinline__ uint32_t make_idesc2(int n, uint32_t sf_id) {
     d |= (uint32_t)(256 >> 4) << 24;    // M = 256 across the CTA pair
     d |= sf_id << 29;
     return d;
-}
-
-// Tile order of the persistent two-CTA kernel.  Tiles that run at the same time (consecutive
-// indices) form a compact block of RASTER_BAND row pairs by as many column tiles, so that the rows of A
-// and B a wave reads are few and each is shared by many CTAs while it is hot in the L2 of their die.
-constexpr int RASTER_BAND = 8;
-__device__ __forceinline__ void tile_coords(int tile, int m_pairs, int n_tiles, int& m_pair, int& n_blk) {
-    const int per_band = RASTER_BAND * n_tiles;
-    const int band = tile / per_band, within = tile - band * per_band;
-    const int rows = min(RASTER_BAND, m_pairs - band * RASTER_BAND);
-    n_blk = within / rows;
-    m_pair = band * RASTER_BAND + (within - n_blk * rows);
 }
 
 template <int BN, int NSTG>

@@ -1,5 +1,6 @@
 // tcgen05 (5th-generation tensor core) wrappers: tensor-memory allocation, fences, commit, accumulator loads /
-// stores, and the shared-memory matrix descriptor of a K-major, 128-byte-swizzled operand.
+// stores, the shared-memory matrix descriptor of a K-major, 128-byte-swizzled operand, and what the GEMM kernels
+// share: the bounded pipeline wait, the CTA-pair (cta_group::2) forms and the tile order.
 #pragma once
 #include "common.cuh"
 
@@ -56,6 +57,90 @@ __device__ __forceinline__ uint64_t make_desc_sw128(uint32_t saddr) {
     d |= (uint64_t)1 << 46;                          // descriptor version (sm_100)
     d |= (uint64_t)2 << 61;                          // SWIZZLE_128B
     return d;
+}
+
+// Bounded wait on wall-clock time (2 s), for the pipeline barriers.
+__device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, int32_t who, volatile int* dead) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*dead) return false;
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023u) == 1023u) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull || *dead) break;
+        }
+    }
+    atomicOr(&g_status, who | 0x100);
+    *dead = 1;
+    return false;
+}
+
+// One lane of a fully converged warp (elect.sync): the issuing warp runs its loop on all 32 lanes so
+// that ring indices, descriptors and addresses stay warp-uniform, and only the tcgen05 instructions
+// themselves are predicated on the elected lane.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred = 0;
+    asm volatile(
+        "{\n\t.reg .b32 rx;\n\t.reg .pred px;\n\t"
+        "elect.sync rx|px, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, px;\n\t}"
+        : "=r"(pred));
+    return pred != 0;
+}
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t mapa_u32(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    // default semantics (as the pipelines of CUTLASS use for consumer -> producer signalling across
+    // CTAs); an explicit .release.cluster here costs ~1500 cycles per arrive
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish2() {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// arrive on a barrier (given by its shared::cluster address) once all MMAs issued so far are done
+__device__ __forceinline__ void tc_commit2(uint32_t cluster_addr) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
+// the same, arriving on the barrier at this shared-memory offset in BOTH CTAs of the pair (one
+// instruction instead of two commits; only the completion signal is multicast, no data copy)
+__device__ __forceinline__ void tc_commit2_pair(uint32_t own_addr) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     own_addr),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+// Tile order of the persistent two-CTA kernel.  Tiles that run at the same time (consecutive
+// indices) form a compact block of RASTER_BAND row pairs by as many column tiles, so that the rows of A
+// and B a wave reads are few and each is shared by many CTAs while it is hot in the L2 of their die.
+constexpr int RASTER_BAND = 8;
+__device__ __forceinline__ void tile_coords(int tile, int m_pairs, int n_tiles, int& m_pair, int& n_blk) {
+    const int per_band = RASTER_BAND * n_tiles;
+    const int band = tile / per_band, within = tile - band * per_band;
+    const int rows = min(RASTER_BAND, m_pairs - band * RASTER_BAND);
+    n_blk = within / rows;
+    m_pair = band * RASTER_BAND + (within - n_blk * rows);
 }
 
 }  // namespace quartet
