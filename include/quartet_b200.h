@@ -45,6 +45,9 @@ enum {
 
 enum { QUARTET_BF16 = 0, QUARTET_F32 = 1 };
 
+/* 8-bit formats */
+enum { QUARTET_E4M3 = 0, QUARTET_E5M2 = 1 };
+
 /* rounding modes of the backward (absmax-scaled) quantizers */
 enum {
     QUARTET_ROUND_NEAREST = 0,    /* AlbertTsengQuantizer(stochastic=False) */
@@ -233,6 +236,59 @@ int quartet_gemm_mxfp4_tn_scatter(const uint8_t* a, const uint8_t* a_sf, const u
 /* out[i] = scale * sum_s slots[s * slot_elems + i], slots added in index order. */
 int quartet_shard_reduce(const float* slots, int32_t n_slots, int64_t slot_elems, float scale, float* out,
                          quartet_stream_t stream);
+
+/*
+ * 8-bit block-scaled linear layer, for the layers that four bits cost too much (the reference keeps its head un-quantized,
+ * src/models/llama.py:197; the notebook's matmul_mxf8_bf16_tn, called in notebooks/benchmark_mxfp4.ipynb:881-973, is the same kind of product).
+ *
+ * quartet_quant_fp8: a block's scale is 2^e, e the least integer with amax <= MAX * 2^e (MAX 448 for e4m3, 57344 for e5m2); a code
+ * is x * 2^-e rounded to the format, ties to even.  Blocks run along the contraction: 1 x 128 (square 0) or 128 x 128 (square 1).
+ *   codes    uint8 [rows, pad128(cols)], the padding zero;  sf: the scale layout above for [rows, pad128(cols)], a block's byte four times
+ *   codes_t  uint8 [cols, pad128(rows)] and sf_t: the same for the transpose of x (blocks along rows)
+ * Either pair may be NULL.  Any rows <= 8388480 and cols.  A block with an infinity or a NaN: scale byte 255, codes NaN.
+ * quartet_dequant_fp8: out [rows, cols] = code * 2^(sf - 127) * scale.
+ */
+int quartet_quant_fp8(const void* x, int x_dtype, int64_t rows, int64_t cols, int fmt, int square, uint8_t* codes, uint8_t* sf, uint8_t* codes_t,
+                      uint8_t* sf_t, quartet_stream_t stream);
+int quartet_dequant_fp8(const uint8_t* codes, const uint8_t* sf, int64_t rows, int64_t cols, int fmt, float scale, void* out, int out_dtype,
+                        quartet_stream_t stream);
+/*
+ * D[M, N] = alpha * A[M, K] . B[N, K]^T on 8-bit codes with one E8M0 scale per 32 values (so also per block of 128), fp32
+ * accumulation, one rounding to d_dtype.  Any M, N >= 1; K a multiple of 128 (zero codes fill up a shorter contraction).
+ * Row r of D starts at d + r * ldd; ldd * (size of d_dtype) must be a multiple of 16; columns N .. ldd - 1 are not written.
+ */
+int quartet_gemm_fp8_tn(const uint8_t* a, const uint8_t* a_sf, int a_fmt, const uint8_t* b, const uint8_t* b_sf, int b_fmt, int64_t M, int64_t N, int64_t K,
+                        float alpha, void* d, int d_dtype, int64_t ldd, quartet_stream_t stream);
+
+/*
+ * Rotary positions (applied to q and k in LlamaAttention, src/models/llama.py:117-158): in every head, pair i of the first `rot` of d values turns
+ * by pos * inv_freq[i], the result times `scale`; the other values are copied.  interleaved 1: pairs (2 i, 2 i + 1), the reference's
+ * layout; 0: pairs (i, i + rot / 2).  inverse 1: by the negative angle (the gradient).
+ * n_seg (1..3) tensors share the launch: segment g is src[g] -> dst[g] with heads[g] heads, element strides strides6[6 g ..] = {src batch,
+ * src token, src head, dst batch, dst token, dst head}, values of a head adjacent; rotate[g] 0 copies it (v).  The five arrays are
+ * HOST arrays.  A dst may be its own src with the same strides; otherwise they must not overlap.
+ * pos: NULL (token t is at offset + t), or int32 / int64 (pos_i64) with strides for batch and token.  inv_freq: double [rot / 2].
+ * rot even, <= min(d, 512); batch * tokens < 2^31.
+ */
+int quartet_rotary(int n_seg, const void* const* src, void* const* dst, const int64_t* strides6, const int32_t* heads, const int32_t* rotate, int dtype,
+                   int64_t batch, int64_t tokens, int64_t d, int64_t rot, int interleaved, const void* pos, int pos_i64, int64_t pos_stride_b,
+                   int64_t pos_stride_t, int64_t offset, const double* inv_freq, float scale, int inverse, quartet_stream_t stream);
+
+/*
+ * Norm over n tensors (clip_grad_norm_ of src/optim/base.py:203-204) and clipping by it, in two launches for any number of tensors up to 768.
+ * grads, numels, dtypes (bf16 / fp32, mixed) are HOST arrays.  kind 0: square root of the sum of squares, taken and added in 64 bits;
+ * kind 1: largest magnitude.  workspace: QUARTET_NORM_PARTIALS doubles of device memory.
+ * quartet_grad_norm: *total = sum of squares (kind 1: the maximum), what ranks that hold different tensors add up (take the largest of);
+ * *norm the norm in fp32.  Either may be NULL.
+ * quartet_clip_grads: outs[i] = grads[i] * c, c = min(1, max_norm / (norm + 1e-6)), NaN where the norm is NaN; outs[i] may be grads[i]; otherwise no
+ * output may share memory with a gradient or another output.  With total (device double, as quartet_grad_norm leaves it) the norm is taken
+ * from there, without it computed first.  norm (fp32, may be NULL) receives it.
+ */
+enum { QUARTET_NORM_PARTIALS = 1024 };
+int quartet_grad_norm(int32_t n, const void* const* grads, const int64_t* numels, const int32_t* dtypes, int kind, double* workspace, double* total,
+                      float* norm, quartet_stream_t stream);
+int quartet_clip_grads(int32_t n, const void* const* grads, void* const* outs, const int64_t* numels, const int32_t* dtypes, const int32_t* out_dtypes,
+                       int kind, double max_norm, const double* total, double* workspace, float* norm, quartet_stream_t stream);
 
 /*
  * Receive buffers other GPUs of the node can map: quartet_peer_alloc allocates `bytes` on the current

@@ -1,0 +1,39 @@
+"""clip_grad_norm_ for the training loop around the quantized layers (src/optim/base.py:203-204 of the reference calls torch's).
+
+One pass over the gradients for the norm and one to scale them, in two launches; nothing waits for the device.  Weights whose gradient lives
+as a shard on each rank (shard.PeerWgradScatter leaves it in `weight.grad_shard`) are clipped by the norm over all ranks' shards.
+"""
+from __future__ import annotations
+
+import torch
+import torch.distributed as dist
+
+from . import ops
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, group=None) -> torch.Tensor:
+    """Scales the gradients in place so that their norm (2 or inf) is at most max_norm; returns the norm before, fp32, on the device.
+
+    A parameter with a `grad_shard` and no `grad` counts as sharded: the squares of shards are summed over the ranks of `group`
+    (every rank then has to make this call); gradients in `.grad` are taken to be the same on every rank.
+    error_if_nonfinite reads the norm back, and raises before anything is scaled."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    whole = [p.grad for p in parameters if p.grad is not None]
+    shards = [p.grad_shard for p in parameters if p.grad is None and getattr(p, "grad_shard", None) is not None]
+    grads = whole + shards
+    if not grads:
+        return torch.zeros(())
+    total = None
+    if shards:
+        if not dist.is_initialized():
+            raise RuntimeError("sharded gradients need an initialised process group")
+        total = ops.grad_norm(shards, norm_type, total=True)
+        dist.all_reduce(total, op=dist.ReduceOp.MAX if norm_type == float("inf") else dist.ReduceOp.SUM, group=group)
+        if whole:
+            rest = ops.grad_norm(whole, norm_type, total=True)
+            total = torch.maximum(total, rest) if norm_type == float("inf") else total + rest
+    elif error_if_nonfinite:
+        total = ops.grad_norm(whole, norm_type, total=True)
+    if error_if_nonfinite and not bool(torch.isfinite(total)):
+        raise RuntimeError(f"the total norm of order {norm_type} of the gradients is not finite")
+    return ops.clip_grads(grads, max_norm, norm_type, total=total)

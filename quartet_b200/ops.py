@@ -403,6 +403,234 @@ def dequant(codes, sf, scale=1.0, dtype=torch.float32):
     return out
 
 
+# ------------------------------------------------------------------------------------------------
+# 8-bit block-scaled linear layer
+# ------------------------------------------------------------------------------------------------
+E4M3, E5M2 = 0, 1
+_F8 = {torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
+
+
+def _f8(dtype) -> int:
+    if dtype not in _F8:
+        raise ValueError(f"8-bit dtype {dtype} not supported (float8_e4m3fn or float8_e5m2)")
+    return _F8[dtype]
+
+
+def _pad128(n: int) -> int:
+    return (n + 127) // 128 * 128
+
+
+def quant_fp8(x, dtype=torch.float8_e4m3fn, square=False, rows=True, transpose=False):
+    """[R, C] (bf16 / fp32) -> (codes [R, pad128(C)], sf blocked u8, codes_t [C, pad128(R)], sf_t): 8-bit values with a power-of-two scale
+    for each block of 128 along the contraction, 1 x 128 or (square) 128 x 128.  `rows` / `transpose` choose the orientations; the
+    other pair is None."""
+    _need_cuda(x)
+    if x.dim() != 2:
+        raise ValueError("x must have two dimensions")
+    if not (rows or transpose):
+        raise ValueError("nothing to quantize: rows and transpose are both False")
+    fmt, (R, K), dev = _f8(dtype), x.shape, x.device
+    codes = sf = codes_t = sf_t = None
+    if rows:
+        codes = torch.empty(R, _pad128(K), dtype=dtype, device=dev)
+        sf = torch.empty(sf_bytes(R, _pad128(K)), dtype=torch.uint8, device=dev)
+    if transpose:
+        codes_t = torch.empty(K, _pad128(R), dtype=dtype, device=dev)
+        sf_t = torch.empty(sf_bytes(K, _pad128(R)), dtype=torch.uint8, device=dev)
+    xdt = _dt(x)
+    if R and K:
+        with _on(dev):
+            rc = _lib.load().quartet_quant_fp8(_ptr(x), xdt, R, K, fmt, int(bool(square)), _ptr(codes), _ptr(sf), _ptr(codes_t), _ptr(sf_t), _stream())
+        _lib.check(rc, "quartet_quant_fp8")
+    return codes, sf, codes_t, sf_t
+
+
+def _need_codes(codes, sf, what):
+    _need_cuda(codes, sf)
+    if codes.dim() != 2 or codes.shape[1] % 128 or sf.dtype != torch.uint8 or sf.numel() != sf_bytes(codes.shape[0], codes.shape[1]):
+        raise ValueError(f"{what}: codes [rows, multiple of 128] and the blocked uint8 scales that belong to them are needed")
+    if sf.device != codes.device:
+        raise ValueError(f"{what}: codes and scales are on different devices")
+
+
+def dequant_fp8(codes, sf, cols=None, scale=1.0, dtype=torch.float32):
+    """Codes of quant_fp8 and their scales -> [rows, cols] values (cols: without the padding; default all columns)."""
+    _need_codes(codes, sf, "dequant_fp8")
+    rows, pitch = codes.shape
+    cols = pitch if cols is None else int(cols)
+    if not 0 <= pitch - cols < 128:
+        raise ValueError(f"{cols} columns do not belong to codes of {pitch}")
+    out = torch.empty(rows, cols, dtype=dtype, device=codes.device)
+    if out.numel():
+        with _on(codes.device):
+            rc = _lib.load().quartet_dequant_fp8(_ptr(codes), _ptr(sf), rows, cols, _f8(codes.dtype), scale, _ptr(out), _out_dt(dtype), _stream())
+        _lib.check(rc, "quartet_dequant_fp8")
+    return out
+
+
+def _padded_out(rows, cols, dtype, dev):
+    """[rows, cols] whose rows start on 16-byte boundaries: a view of a wider buffer where cols does not fill one."""
+    per = 16 // dtype.itemsize
+    pitch = (cols + per - 1) // per * per
+    out = torch.empty(rows, pitch, dtype=dtype, device=dev)
+    return (out if pitch == cols else out[:, :cols]), pitch
+
+
+def gemm_fp8_tn(a, a_sf, b, b_sf, alpha=1.0, out_dtype=torch.bfloat16):
+    """D[M, N] = alpha * A[M, K] . B[N, K]^T on 8-bit codes with blocked E8M0 scales, as quant_fp8 makes them.  Where a row of D is no
+    multiple of 16 bytes, D is a view of a buffer whose rows are."""
+    _need_codes(a, a_sf, "gemm_fp8_tn (a)")
+    _need_codes(b, b_sf, "gemm_fp8_tn (b)")
+    (M, K), N = a.shape, b.shape[0]
+    if b.shape[1] != K:
+        raise ValueError(f"contraction extents differ: {K} vs {b.shape[1]}")
+    if a.device != b.device:
+        raise ValueError("operands are on different devices")
+    fa, fb, dd = _f8(a.dtype), _f8(b.dtype), _out_dt(out_dtype)
+    if M == 0 or N == 0 or K == 0:
+        return torch.zeros(M, N, dtype=out_dtype, device=a.device)
+    out, pitch = _padded_out(M, N, out_dtype, a.device)
+    with _on(a.device):
+        rc = _lib.load().quartet_gemm_fp8_tn(_ptr(a), _ptr(a_sf), fa, _ptr(b), _ptr(b_sf), fb, M, N, K, alpha, _ptr(out), dd, pitch, _stream())
+    _lib.check(rc, "quartet_gemm_fp8_tn")
+    return out
+
+
+def linear_fp8(x, w, w_sf, out_dtype=None):
+    """x [..., K] times a packed weight (codes [N, pad128(K)] and scales of quant_fp8(weight, square=True)) -> [..., N]: x is quantized in
+    blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear."""
+    _need_codes(w, w_sf, "linear_fp8")
+    K = x.shape[-1]
+    if _pad128(K) != w.shape[1]:
+        raise ValueError(f"x has {K} columns, the weight {w.shape[1]}")
+    x2 = x.reshape(-1, K)
+    xc, xs, _, _ = quant_fp8(x2 if x2.is_contiguous() else x2.contiguous())
+    y = gemm_fp8_tn(xc, xs, w, w_sf, out_dtype=out_dtype or x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+
+
+# ------------------------------------------------------------------------------------------------
+# rotary positions
+# ------------------------------------------------------------------------------------------------
+def rotary(segments, inv_freq, positions=None, offset=0, interleaved=True, scale=1.0, inverse=False):
+    """Turns (or copies) up to three tensors in one launch.  segments: (src, dst, rotate), src and dst [batch, tokens, heads, d] views of any
+    strides whose last axis is contiguous.  positions: int32 / int64 [tokens] or [batch, tokens], or None for offset, offset + 1, ...
+    inv_freq: float64 [rot / 2].  A dst may be its own src; otherwise they must not overlap."""
+    n = len(segments)
+    x0 = segments[0][0]
+    B, T, _, d = x0.shape
+    dev, dt = x0.device, _dt(x0)
+    ints = []
+    for src, dst, _ in segments:
+        if not (src.is_cuda and src.device == dev and dst.device == dev):
+            raise ValueError("tensors must live on one CUDA device")
+        if src.dtype != x0.dtype or dst.dtype != x0.dtype or src.shape != dst.shape or src.dim() != 4 or src.shape[:2] != x0.shape[:2] or src.shape[3] != d:
+            raise ValueError("segments must agree in dtype, batch, tokens and d")
+        if d > 1 and (src.stride(3) != 1 or dst.stride(3) != 1):
+            raise ValueError("the values of a head must be adjacent")
+        ints += [*src.stride()[:3], *dst.stride()[:3]]
+    if not (inv_freq.is_cuda and inv_freq.device == dev and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+        raise ValueError("inv_freq must be a contiguous float64 vector on the tensors' device")
+    pos_ptr, i64, pb, pt = None, 0, 0, 0
+    if positions is not None:
+        if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("positions must be int32 or int64 on the tensors' device")
+        if tuple(positions.shape) == (T,):
+            pt = positions.stride(0)
+        elif tuple(positions.shape) == (B, T):
+            pb, pt = positions.stride()
+        else:
+            raise ValueError(f"positions must have shape ({T},) or ({B}, {T}), not {tuple(positions.shape)}")
+        pos_ptr, i64 = _ptr(positions), int(positions.dtype == torch.int64)
+    srcs = (C.c_void_p * n)(*[s.data_ptr() for s, _, _ in segments])
+    dsts = (C.c_void_p * n)(*[t.data_ptr() for _, t, _ in segments])
+    if B * T == 0:
+        return
+    with _on(dev):
+        rc = _lib.load().quartet_rotary(n, srcs, dsts, (C.c_int64 * (6 * n))(*ints), (C.c_int32 * n)(*[s.shape[2] for s, _, _ in segments]),
+                                        (C.c_int32 * n)(*[int(bool(r)) for _, _, r in segments]), dt, B, T, d, 2 * inv_freq.numel(), int(bool(interleaved)),
+                                        pos_ptr, i64, pb, pt, int(offset), _ptr(inv_freq), float(scale), int(bool(inverse)), _stream())
+    _lib.check(rc, "quartet_rotary")
+
+
+# ------------------------------------------------------------------------------------------------
+# norm over many tensors, and clipping by it
+# ------------------------------------------------------------------------------------------------
+NORM_PARTIALS = 1024
+_LIST_DT = {torch.bfloat16: BF16, torch.float32: F32}
+
+
+def _dense(t) -> bool:
+    """Whether the elements fill one stretch of memory, in whatever order of the axes."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+def _tensor_list(ts, dev, what):
+    for t in ts:
+        if t.device != dev or t.dtype not in _LIST_DT or not _dense(t):
+            raise ValueError(f"{what} must be dense bf16 or fp32 tensors on one CUDA device")
+    n = len(ts)
+    return (C.c_void_p * n)(*[t.data_ptr() for t in ts]), (C.c_int64 * n)(*[t.numel() for t in ts]), (C.c_int32 * n)(*[_LIST_DT[t.dtype] for t in ts])
+
+
+def _norm_kind(norm_type) -> int:
+    if norm_type == 2:
+        return 0
+    if norm_type == float("inf"):
+        return 1
+    raise ValueError(f"norm_type must be 2 or inf, not {norm_type}")
+
+
+def grad_norm(tensors, norm_type=2.0, total=False):
+    """Norm over all elements of the tensors (bf16 / fp32, mixed): fp32 scalar on their device.  total=True returns instead what ranks that hold
+    different tensors combine: the float64 sum of squares, shape [1] (for the maximum norm, the maximum)."""
+    tensors, kind = list(tensors), _norm_kind(norm_type)
+    if not tensors or not tensors[0].is_cuda:
+        raise ValueError("need at least one tensor, on a CUDA device")
+    dev = tensors[0].device
+    ptrs, numels, dts = _tensor_list(tensors, dev, "tensors")
+    work = torch.empty(NORM_PARTIALS + 1, dtype=torch.float64, device=dev)
+    out = work[NORM_PARTIALS:] if total else torch.empty((), dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = _lib.load().quartet_grad_norm(len(tensors), ptrs, numels, dts, kind, _ptr(work), _ptr(out) if total else None, None if total else _ptr(out),
+                                           _stream())
+    _lib.check(rc, "quartet_grad_norm")
+    return out
+
+
+def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
+    """Scales the tensors by min(1, max_norm / (norm + 1e-6)), in place or into `out` (a tensor for each, fp32 or bf16, of its shape and strides);
+    returns the norm before (fp32 scalar on the device; nothing waits for it).  total: a float64 [1] as grad_norm(..., total=True) returns it, e.g.
+    summed over ranks, to use in place of the tensors' own."""
+    tensors, kind = list(tensors), _norm_kind(norm_type)
+    if not tensors or not tensors[0].is_cuda:
+        raise ValueError("need at least one tensor, on a CUDA device")
+    dev = tensors[0].device
+    ptrs, numels, dts = _tensor_list(tensors, dev, "tensors")
+    optrs, odts = ptrs, dts
+    if out is not None:
+        out = list(out)
+        if len(out) != len(tensors) or any(o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))
+                                           for o, t in zip(out, tensors)):
+            raise ValueError("out must hold a tensor of the same shape and strides for each of the tensors")
+        optrs, _, odts = _tensor_list(out, dev, "out")
+    if total is not None and not (total.is_cuda and total.device == dev and total.dtype == torch.float64 and total.numel() == 1):
+        raise ValueError("total must be one float64 value on the tensors' device")
+    work = torch.empty(NORM_PARTIALS, dtype=torch.float64, device=dev) if total is None else None
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = _lib.load().quartet_clip_grads(len(tensors), ptrs, optrs, numels, dts, odts, kind, float(max_norm), _ptr(total), _ptr(work), _ptr(norm), _stream())
+    _lib.check(rc, "quartet_clip_grads")
+    return norm
+
+
 def device_status() -> int:
     """Fault word of the current device (0 = no kernel ever gave up on a bounded wait); clears it."""
     st = C.c_int32(0)

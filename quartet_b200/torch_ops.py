@@ -419,3 +419,173 @@ def _swiglu_linear_backward(ctx, e, *unused):
 
 
 torch.library.register_autograd("quartet_b200::swiglu_linear_fwd", _swiglu_linear_backward, setup_context=_swiglu_linear_setup)
+
+
+# ------------------------------------------------------------------------------------------------
+# rotary positions
+# ------------------------------------------------------------------------------------------------
+def split_heads(qkv: Tensor, n_head: int, n_kv_head: int, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
+                head_major: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """Packed projection -> q, k (turned) and v in one launch."""
+    qkv = qkv if qkv.stride(-1) == 1 else qkv.contiguous()
+    b, t, w = qkv.shape
+    d = w // (n_head + 2 * n_kv_head)
+    outs, segments, at = [], [], 0
+    for i, h in enumerate((n_head, n_kv_head, n_kv_head)):
+        y = qkv.new_empty((b, h, t, d) if head_major else (b, t, h, d))
+        src = qkv[..., at:at + h * d].unflatten(-1, (h, d))
+        outs.append(y)
+        segments.append((src, y.transpose(1, 2) if head_major else y, i < 2))
+        at += h * d
+    ops.rotary(segments, inv_freq, positions, offset, interleaved, scale)
+    return outs[0], outs[1], outs[2]
+
+
+def join_heads(dq: Tensor, dk: Tensor, dv: Tensor, head_major: bool, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool,
+               scale: float) -> Tensor:
+    """The gradient of split_heads: gradients of q, k, v (any strides) -> the packed one."""
+    gs = [g.transpose(1, 2) if head_major else g for g in (dq, dk, dv)]
+    b, t, _, d = gs[0].shape
+    out = dq.new_empty(b, t, sum(g.shape[2] for g in gs) * d)
+    segments, at = [], 0
+    for i, g in enumerate(gs):
+        g = g if g.stride(-1) == 1 or d == 1 else g.contiguous()
+        h = g.shape[2]
+        segments.append((g, out[..., at:at + h * d].unflatten(-1, (h, d)), i < 2))
+        at += h * d
+    ops.rotary(segments, inv_freq, positions, offset, interleaved, scale, inverse=True)
+    return out
+
+
+@torch.library.custom_op("quartet_b200::rotary", mutates_args=())
+def rotary(x: Tensor, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float, inverse: bool) -> Tensor:
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    ops.rotary([(x, y, True)], inv_freq, positions, offset, interleaved, scale, inverse)
+    return y
+
+
+@rotary.register_fake
+def _(x, inv_freq, positions, offset, interleaved, scale, inverse):
+    return x.new_empty(x.shape)
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, inv_freq, positions, *ctx.args = inputs
+    ctx.save_for_backward(inv_freq, positions)
+
+
+def _rotary_backward(ctx, g):
+    inv_freq, positions = ctx.saved_tensors
+    offset, interleaved, scale, inverse = ctx.args
+    return torch.ops.quartet_b200.rotary(g, inv_freq, positions, offset, interleaved, scale, not inverse), None, None, None, None, None, None
+
+
+torch.library.register_autograd("quartet_b200::rotary", _rotary_backward, setup_context=_rotary_setup)
+
+
+@torch.library.custom_op("quartet_b200::rotary_qkv", mutates_args=())
+def rotary_qkv(qkv: Tensor, n_head: int, n_kv_head: int, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
+               head_major: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    return split_heads(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
+
+
+@rotary_qkv.register_fake
+def _(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major):
+    b, t, w = qkv.shape
+    d = w // (n_head + 2 * n_kv_head)
+    return tuple(qkv.new_empty((b, h, t, d) if head_major else (b, t, h, d)) for h in (n_head, n_kv_head, n_kv_head))
+
+
+@torch.library.custom_op("quartet_b200::rotary_qkv_bwd", mutates_args=())
+def rotary_qkv_bwd(dq: Tensor, dk: Tensor, dv: Tensor, head_major: bool, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool,
+                   scale: float) -> Tensor:
+    return join_heads(dq, dk, dv, head_major, inv_freq, positions, offset, interleaved, scale)
+
+
+@rotary_qkv_bwd.register_fake
+def _(dq, dk, dv, head_major, inv_freq, positions, offset, interleaved, scale):
+    h, t = (1, 2) if head_major else (2, 1)
+    return dq.new_empty(dq.shape[0], dq.shape[t], (dq.shape[h] + dk.shape[h] + dv.shape[h]) * dq.shape[3])
+
+
+def _rotary_qkv_setup(ctx, inputs, output):
+    _, _, _, inv_freq, positions, offset, interleaved, scale, head_major = inputs
+    ctx.save_for_backward(inv_freq, positions)
+    ctx.args, ctx.head_major = (offset, interleaved, scale), head_major
+
+
+def _rotary_qkv_backward(ctx, dq, dk, dv):
+    inv_freq, positions = ctx.saved_tensors
+    return (torch.ops.quartet_b200.rotary_qkv_bwd(dq, dk, dv, ctx.head_major, inv_freq, positions, *ctx.args),) + (None,) * 8
+
+
+torch.library.register_autograd("quartet_b200::rotary_qkv", _rotary_qkv_backward, setup_context=_rotary_qkv_setup)
+
+
+# ------------------------------------------------------------------------------------------------
+# the 8-bit block-scaled linear layer
+# ------------------------------------------------------------------------------------------------
+@torch.library.custom_op("quartet_b200::fp8_linear_fwd", mutates_args=())
+def fp8_linear_fwd(x: Tensor, w: Tensor, grad_dtype: torch.dtype, out_dtype: torch.dtype, need_dx: bool,
+                   need_dw: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """y = Q(x) Q(w)^T and what its backward needs: the codes and scales of x and w transposed (empty where not needed)."""
+    K = w.shape[1]
+    x2 = x.reshape(-1, K)
+    xc, xs, xtc, xts = ops.quant_fp8(x2 if x2.is_contiguous() else x2.contiguous(), transpose=need_dw)
+    wc, ws, wtc, wts = ops.quant_fp8(w if w.is_contiguous() else w.contiguous(), square=True, transpose=need_dx)
+    y = ops.gemm_fp8_tn(xc, xs, wc, ws, out_dtype=out_dtype).reshape(*x.shape[:-1], w.shape[0])
+    e8, e1 = xc.new_empty((0, 0)), xs.new_empty((0,))
+    return y.contiguous(), (e8 if xtc is None else xtc), (e1 if xts is None else xts), (e8.clone() if wtc is None else wtc), (e1.clone() if wts is None else wts)
+
+
+@fp8_linear_fwd.register_fake
+def _(x, w, grad_dtype, out_dtype, need_dx, need_dw):
+    N, K = w.shape
+    m, f8 = x.numel() // K, torch.float8_e4m3fn
+    mp, np_ = _pad128(m), _pad128(N)
+    return (x.new_empty((*x.shape[:-1], N), dtype=out_dtype),
+            x.new_empty((K, mp) if need_dw else (0, 0), dtype=f8), _u8(x, _sf_bytes(K, mp) if need_dw else 0),
+            x.new_empty((K, np_) if need_dx else (0, 0), dtype=f8), _u8(x, _sf_bytes(K, np_) if need_dx else 0))
+
+
+@torch.library.custom_op("quartet_b200::fp8_linear_bwd", mutates_args=())
+def fp8_linear_bwd(e: Tensor, xtc: Tensor, xts: Tensor, wtc: Tensor, wts: Tensor, grad_dtype: torch.dtype, x_dtype: torch.dtype, w_dtype: torch.dtype,
+                   need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
+    """dx [m, K] = Q(e) Q(w) and dw [N, K] = Qt(e)^T Qt(x); empty where not needed."""
+    N = e.shape[-1]
+    e2 = e.reshape(-1, N)
+    if e2.dtype not in (torch.bfloat16, torch.float32):
+        e2 = e2.float()
+    ec, es, etc, ets = ops.quant_fp8(e2 if e2.is_contiguous() else e2.contiguous(), grad_dtype, rows=need_dx, transpose=need_dw)
+    dx = ops.gemm_fp8_tn(ec, es, wtc, wts, out_dtype=x_dtype).contiguous() if need_dx else e.new_empty((0,), dtype=x_dtype)
+    dw = ops.gemm_fp8_tn(etc, ets, xtc, xts, out_dtype=w_dtype).contiguous() if need_dw else e.new_empty((0,), dtype=w_dtype)
+    ops.raise_on_fault("8-bit linear backward")  # only with QUARTET_CHECK_FAULTS=1
+    return dx, dw
+
+
+@fp8_linear_bwd.register_fake
+def _(e, xtc, xts, wtc, wts, grad_dtype, x_dtype, w_dtype, need_dx, need_dw):
+    N = e.shape[-1]
+    m = e.numel() // N
+    dx = e.new_empty((m, wtc.shape[0]) if need_dx else (0,), dtype=x_dtype)
+    dw = e.new_empty((N, xtc.shape[0]) if need_dw else (0,), dtype=w_dtype)
+    return dx, dw
+
+
+def _fp8_linear_setup(ctx, inputs, output):
+    x, w, grad_dtype, _, need_dx, need_dw = inputs
+    ctx.save_for_backward(*output[1:])
+    ctx.x_shape, ctx.args = x.shape, (grad_dtype, x.dtype, w.dtype, need_dx, need_dw)
+    ctx.set_materialize_grads(False)
+
+
+def _fp8_linear_backward(ctx, e, *unused):
+    if e is None:
+        return (None,) * 6
+    dx, dw = torch.ops.quartet_b200.fp8_linear_bwd(e, *ctx.saved_tensors, *ctx.args)
+    need_dx, need_dw = ctx.args[3:]
+    return (dx.reshape(ctx.x_shape) if need_dx else None), (dw if need_dw else None), None, None, None, None
+
+
+torch.library.register_autograd("quartet_b200::fp8_linear_fwd", _fp8_linear_backward, setup_context=_fp8_linear_setup)
