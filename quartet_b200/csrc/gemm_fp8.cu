@@ -251,6 +251,346 @@ static int launch_split(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8
     return check_cuda(cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, p, splits), "gemm_fp8 launch");
 }
 
+// ---------------------------------------------------------------------------
+// CTA pairs (cta_group::2): 256 x 256 results a pair, persistent
+// ---------------------------------------------------------------------------
+struct PairCfg {
+    static constexpr int BN = 256;
+    static constexpr int A_BYTES = 128 * 128;                // this CTA's rows of A, 128 values
+    static constexpr int B_BYTES = 128 * 128;                // this CTA's half of B's rows
+    static constexpr int SFA_BYTES = 512, SFB_BYTES = 1024;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+    static constexpr int NBUF = 1;                           // staging buffers of an epilogue warp, 4 KB each
+    static constexpr int STG_BYTES = 8 * NBUF * 4096;
+    static constexpr int STAGES = (232448 - STG_BYTES - 512) / STAGE_BYTES;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + STG_BYTES + 512;
+    // Consecutive tiles accumulate in columns [0, 256) and [128, 384): the 128 they share are drained into registers first, so
+    // that the next tile's products start while the rest of the epilogue still runs.
+    static constexpr int ACC_SHIFT = 128;
+    static constexpr int SF_COL0 = 384, SF_COLS = 12, SF_SLOTS = 4;
+    static_assert(SF_COL0 + SF_SLOTS * SF_COLS <= 512, "tensor memory capacity");
+    static_assert(SF_SLOTS < STAGES, "scale slots are recycled through the stage barriers");
+};
+constexpr int PAIR_THREADS = 512;  // warps 0, 10, 15 issue copies (A, B, scales), 1 the MMAs, 6-9 feed scales, 2-5 and 11-14 drain
+
+__device__ __forceinline__ void tc_mma2_mxf8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+}
+
+// 32 rows x 64 columns of results, one row per thread, through 4 KB of swizzled staging to global memory: one tensor store of 64 bf16
+// columns or two of 32 fp32 columns, 128 bytes a row.  The tensor map clips what lies outside D, but only to whole 16-byte units of a row
+// (measured: the rest of the last unit is written as zeros), so a block that ends inside one is written value by value.
+template <int NBUF>
+__device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const uint32_t (&r1)[32], const Fp8GemmParams& p, const CUtensorMap* tm_d, int row0,
+                                              int col, uint8_t* stg, uint32_t& n_stores, int lane) {
+    if (col + 64 > p.N && p.N % (p.d_f32 ? 4 : 8) != 0) {
+        const int64_t row = (int64_t)row0 + lane;
+        const int n = (int)(p.N - col);
+        if (row < p.M) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+                if (i >= n) break;
+                const float v = __uint_as_float(i < 32 ? r0[i & 31] : r1[i & 31]) * p.alpha;
+                if (p.d_f32)
+                    static_cast<float*>(p.d)[row * p.ldd + col + i] = v;
+                else
+                    static_cast<__nv_bfloat16*>(p.d)[row * p.ldd + col + i] = __float2bfloat16_rn(v);
+            }
+        }
+        return;
+    }
+    auto slot = [&]() -> uint8_t* {
+        uint8_t* buf = stg + (n_stores % NBUF) * 4096;
+        ++n_stores;
+        if (lane == 0) { if (NBUF == 2) bulk_wait_read1(); else bulk_wait_read0(); }
+        __syncwarp();
+        return buf;
+    };
+    auto send = [&](uint8_t* buf, int c) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(tm_d, c, row0, buf);
+            bulk_commit();
+        }
+    };
+    if (p.d_f32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint8_t* buf = slot();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(h ? r1[4 * j + k] : r0[4 * j + k]) * p.alpha;
+                *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            send(buf, col + 32 * h);
+        }
+    } else {
+        uint8_t* buf = slot();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = (8 * j + 2 * k) & 31;
+                const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(j < 4 ? r0[i] : r1[i]) * p.alpha, __uint_as_float(j < 4 ? r0[i + 1] : r1[i + 1]) * p.alpha);
+                w[k] = *reinterpret_cast<const uint32_t*>(&t);
+            }
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        send(buf, col);
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_d,
+                         const __grid_constant__ CUtensorMap tm_sfb, const Fp8GemmParams p) {
+    using C = PairCfg;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) atomicOr(&g_status, WAIT_GEMM_ALIGN | 0x100);
+        return;
+    }
+    uint8_t* s_a = smem;
+    uint8_t* s_b = s_a + C::STAGES * C::A_BYTES;
+    uint8_t* s_stg = s_b + C::STAGES * C::B_BYTES;
+    uint8_t* s_sfb = s_stg + C::STG_BYTES;
+    uint8_t* s_sfa = s_sfb + C::STAGES * C::SFB_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_sfa + C::STAGES * C::SFA_BYTES);
+    uint64_t* full = bars;                       // local: this CTA's copies of a stage have landed
+    uint64_t* empty = full + C::STAGES;          // local: the pair's MMAs are done with the stage
+    uint64_t* sf_full = empty + C::STAGES;       // leader: 8 feeder warps (both CTAs) have fed the stage
+    uint64_t* sf_land = sf_full + C::STAGES;     // local: the stage's scale blocks have landed
+    uint64_t* sf_free = sf_land + C::STAGES;     // local: the 4 feeder warps hold the stage's scales in registers
+    uint64_t* acc_full = sf_free + C::STAGES;    // local: accumulator complete
+    uint64_t* acc_empty = acc_full + 1;          // leader: 16 epilogue warps (both CTAs) have drained the shared columns
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_empty + 1);
+    volatile int* dead = reinterpret_cast<volatile int*>(s_tmem + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(&full[i], 2);
+            mbar_init(&empty[i], 1);
+            mbar_init(&sf_full[i], 8);
+            mbar_init(&sf_land[i], 1);
+            mbar_init(&sf_free[i], 4);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 16);
+        *dead = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm_a);
+        prefetch_tmap(&tm_b);
+        prefetch_tmap(&tm_d);
+        prefetch_tmap(&tm_sfb);
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_alloc2(s_tmem, 512);
+        tmem_relinquish2();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *s_tmem;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int m_pairs = (int)((p.M + 255) / 256), n_tiles = (int)((p.N + 255) / 256);
+    const int m_blocks = (int)((p.M + 127) / 128);
+    const int n_tiles_total = m_pairs * n_tiles;
+    const int n_clusters = gridDim.x >> 1, cluster_id = blockIdx.x >> 1;
+    const int k_stages = p.k_chunks;
+
+    if (warp == 0 || warp == 10 || warp == 15) {
+        if (lane == 0) {
+            const int role = warp == 0 ? 0 : (warp == 10 ? 1 : 2);
+            const uint64_t keep = l2_policy_evict_last();
+            uint32_t s = 0, ph = 0;
+            for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
+                int m_pair, n_blk;
+                tile_coords(tile, m_pairs, n_tiles, m_pair, n_blk);
+                const int m_blk = m_pair * 2 + (int)rank;
+                const int n0 = n_blk * C::BN;
+                // a second row block past the last one reads zero rows; its scales are the last block's, there being none of its own
+                const uint8_t* sfa_src = p.a_sf + (int64_t)min(m_blk, m_blocks - 1) * p.k_chunks * 512;
+                for (int ks = 0; ks < k_stages; ++ks) {
+                    if (!gemm_wait(role == 2 ? &sf_free[s] : &empty[s], ph ^ 1, WAIT_GEMM_EMPTY, dead)) break;
+                    if (role == 0) {
+                        mbar_arrive_expect_tx(&full[s], C::A_BYTES);
+                        tma_load_2d_hint(s_a + s * C::A_BYTES, &tm_a, ks * 128, m_blk * 128, &full[s], keep);
+                    } else if (role == 1) {
+                        mbar_arrive_expect_tx(&full[s], C::B_BYTES);
+                        tma_load_2d_hint(s_b + s * C::B_BYTES, &tm_b, ks * 128, n0 + (int)rank * 128, &full[s], keep);
+                    } else {
+                        mbar_arrive_expect_tx(&sf_land[s], C::SFA_BYTES + C::SFB_BYTES);
+                        bulk_load_hint(s_sfa + s * C::SFA_BYTES, sfa_src + (int64_t)ks * 512, C::SFA_BYTES, &sf_land[s], keep);
+                        tma_load_2d_hint(s_sfb + s * C::SFB_BYTES, &tm_sfb, ks * 128, n0 / 128, &sf_land[s], keep);
+                    }
+                    if (++s == C::STAGES) s = 0, ph ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (leader) {
+            uint32_t s = 0, ph = 0, slot = 0, aph = 0, acc_it = 0;
+            const uint32_t id0 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 0), id1 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 1);
+            const uint32_t id2 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 2), id3 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 3);
+            const uint32_t a_base = smem_u32(s_a), b_base = smem_u32(s_b);
+            const uint32_t empty_own = smem_u32(&empty[0]), accf_own = smem_u32(acc_full);
+            for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
+                if (!gemm_wait(acc_empty, aph ^ 1, WAIT_GEMM_ACC_EMPTY, dead)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (acc_it & 1) * C::ACC_SHIFT;
+                ++acc_it;
+                for (int ks = 0; ks < k_stages; ++ks) {
+                    if (!gemm_wait(&sf_full[s], ph, WAIT_GEMM_SF, dead)) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t sf = tmem_base + C::SF_COL0 + slot * C::SF_COLS;
+                        const uint64_t ad = make_desc_sw128(a_base + s * C::A_BYTES), bd = make_desc_sw128(b_base + s * C::B_BYTES);
+                        tc_mma2_mxf8(d_tmem, ad, bd, id0, sf, sf + 4, ks != 0);
+                        tc_mma2_mxf8(d_tmem, ad + 2, bd + 2, id1, sf | (1u << 30), (sf + 4) | (1u << 30), 1);
+                        tc_mma2_mxf8(d_tmem, ad + 4, bd + 4, id2, sf | (2u << 30), (sf + 4) | (2u << 30), 1);
+                        tc_mma2_mxf8(d_tmem, ad + 6, bd + 6, id3, sf | (3u << 30), (sf + 4) | (3u << 30), 1);
+                        tc_commit2_pair(empty_own + s * 8);
+                    }
+                    __syncwarp();
+                    if (++s == C::STAGES) s = 0, ph ^= 1;
+                    if (++slot == C::SF_SLOTS) slot = 0;
+                }
+                if (elect_one()) tc_commit2_pair(accf_own);
+                __syncwarp();
+                aph ^= 1;
+            }
+        }
+    } else if (warp >= 6 && warp <= 9) {
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t it = 0;
+        for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
+            for (int ks = 0; ks < k_stages; ++ks, ++it) {
+                const int s = it % C::STAGES;
+                const uint32_t ph = (it / C::STAGES) & 1;
+                if (!gemm_wait(&sf_land[s], ph, WAIT_GEMM_FULL, dead)) break;
+                const uint32_t sf = tmem_base + lane_base + C::SF_COL0 + (it % C::SF_SLOTS) * C::SF_COLS;
+                const uint4 va = *reinterpret_cast<const uint4*>(s_sfa + s * C::SFA_BYTES + lane * 16);
+                const uint4 v0 = *reinterpret_cast<const uint4*>(s_sfb + s * C::SFB_BYTES + lane * 16);
+                const uint4 v1 = *reinterpret_cast<const uint4*>(s_sfb + s * C::SFB_BYTES + 512 + lane * 16);
+                const uint32_t ra[8] = {va.x, va.y, va.z, va.w, 0, 0, 0, 0}, rb[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sf_free[s]);
+                if (it >= (uint32_t)C::SF_SLOTS) {
+                    const uint32_t pit = it - C::SF_SLOTS;
+                    if (!gemm_wait(&empty[pit % C::STAGES], (pit / C::STAGES) & 1, WAIT_GEMM_EMPTY, dead)) break;
+                    tc_fence_after();
+                }
+                tc_st4(sf, ra);
+                tc_st8(sf + 4, rb);
+                tc_wait_st();
+                tc_fence_before();
+                if (!gemm_wait(&full[s], ph, WAIT_GEMM_FULL, dead)) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&sf_full[s]), 0));
+            }
+        }
+    } else {
+        // two warps per lane quadrant; each takes one 64-column block of the shared half of the accumulator, then one of the other half
+        const int q = warp & 3, par = warp >= 11 ? 1 : 0;
+        uint8_t* stg = s_stg + (par * 4 + q) * (C::NBUF * 4096);
+        uint32_t acc_it = 0, n_stores = 0;
+        for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters, ++acc_it) {
+            int m_pair, n_blk;
+            tile_coords(tile, m_pairs, n_tiles, m_pair, n_blk);
+            const int n0 = n_blk * C::BN;
+            const int row0 = (m_pair * 2 + (int)rank) * 128 + q * 32;
+            if (!gemm_wait(acc_full, acc_it & 1, WAIT_GEMM_ACC_FULL, dead)) break;
+            tc_fence_after();
+            const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (acc_it & 1) * C::ACC_SHIFT;
+            const int first = (acc_it & 1) ? 0 : 128;         // the half that the next tile's accumulator overlaps
+            const int c0 = first + par * 64, c1 = (first ^ 128) + par * 64;
+            uint32_t r0[32], r1[32];
+            tc_ld32(t0 + c0, r0);
+            tc_ld32(t0 + c0 + 32, r1);
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty), 0));
+            const bool rows = row0 < p.M;
+            if (rows && n0 + c0 < p.N) store_block64<C::NBUF>(r0, r1, p, &tm_d, row0, n0 + c0, stg, n_stores, lane);
+            tc_ld32(t0 + c1, r0);
+            tc_ld32(t0 + c1 + 32, r1);
+            tc_wait_ld();
+            if (rows && n0 + c1 < p.N) store_block64<C::NBUF>(r0, r1, p, &tm_d, row0, n0 + c1, stg, n_stores, lane);
+            tc_fence_before();  // all of this tile's tensor-memory reads are complete before the warp's next arrive
+        }
+        if (lane == 0) bulk_wait0();
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*dead)
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc2(tmem_base, 512);
+    }
+}
+
+static int launch_pair(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t stream) {
+    using C = PairCfg;
+    CUtensorMap tm_a, tm_b, tm_d, tm_sfb;
+    int rc = make_tmap_2d(&tm_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.M, K, 128, 128, 3);
+    if (rc) return rc;
+    if ((rc = make_tmap_2d(&tm_b, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.N, K, 128, 128, 3))) return rc;
+    if (p.d_f32)
+        rc = make_tmap_2d(&tm_d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.N, p.M, (uint64_t)p.ldd * 4, 32, 32, 3);
+    else
+        rc = make_tmap_2d(&tm_d, p.d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.N, p.M, (uint64_t)p.ldd * 2, 64, 32, 3);
+    if (rc) return rc;
+    // B's scales as 32-bit words: a row for each 128-row block, 128 words a chunk; a stage takes one chunk of two row blocks
+    if ((rc = make_tmap_2d(&tm_sfb, p.b_sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (uint64_t)p.k_chunks * 128, (uint64_t)((p.N + 127) / 128),
+                           (uint64_t)p.k_chunks * 512, 128, 2, 0)))
+        return rc;
+    auto kern = gemm_fp8_pair_kernel;
+    static thread_local int smem_set = -1;
+    if ((rc = set_max_smem_once(kern, C::SMEM, smem_set))) return rc;
+    int dev = 0, sms = 0;
+    if ((rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice"))) return rc;
+    if ((rc = device_sm_count(&sms))) return rc;
+    // a persistent kernel launches no more clusters than can be resident at once
+    static thread_local int cached_dev = -1, cached_clusters = 0;
+    if (cached_dev != dev) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)sms), cfg.blockDim = dim3(PAIR_THREADS), cfg.dynamicSmemBytes = C::SMEM;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr, cfg.numAttrs = 1;
+        int n = 0;
+        if ((rc = check_cuda(cudaOccupancyMaxActiveClusters(&n, kern, &cfg), "cudaOccupancyMaxActiveClusters"))) return rc;
+        if (n < 1) return fail(QUARTET_E_CUDA, "no CTA pair can be resident");
+        cached_dev = dev, cached_clusters = n;
+    }
+    const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int clusters = (int)(tiles < cached_clusters ? tiles : cached_clusters);
+    return check_cuda(launch_pdl(kern, dim3(clusters * 2), dim3(PAIR_THREADS), C::SMEM, stream, tm_a, tm_b, tm_d, tm_sfb, p), "gemm_fp8 launch");
+}
+
 QUARTET_DEFINE_STATUS_READER(status_gemm_fp8)
 
 }  // namespace quartet
@@ -278,5 +618,6 @@ extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_tn(const 
     p.a_e5m2 = a_fmt, p.b_e5m2 = b_fmt;
     p.alpha = alpha, p.d = d, p.d_f32 = d_dtype == QUARTET_F32;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (M >= 256 && N >= 256) return launch_pair(a, b, K, p, s);
     return launch_split<128>(a, b, K, p, 1, s);
 }
