@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 
 import torch
 
@@ -14,6 +15,7 @@ ROUND_NEAREST, ROUND_SR_PHILOX, ROUND_SR_NOISE, ROUND_SR_TLRAND = 0, 1, 2, 3
 QUEST_GAUSSIAN_SCALE = 2.92247856 / 6.0
 HAD_SCALE_BF16 = 0.1767578125  # bf16(32 ** -0.5)
 HAD_SCALE_F32 = 0.17677669529663687
+_LIST_DT = {torch.bfloat16: BF16, torch.float32: F32}
 SR_OPERAND_SCALE = 4.0 / 3.0  # each absmax-quantized operand carries this factor outside its scale bytes
 
 
@@ -38,7 +40,8 @@ def _ptr(t):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the current device's stream as an address: building a torch.cuda.Stream object costs 3 us a call, this 0.1
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 class _NoSwitch:
@@ -516,48 +519,62 @@ def rotary(segments, inv_freq, positions=None, offset=0, interleaved=True, scale
     """Turns (or copies) up to three tensors in one launch.  segments: (src, dst, rotate), src and dst [batch, tokens, heads, d] views of any
     strides whose last axis is contiguous.  positions: int32 / int64 [tokens] or [batch, tokens], or None for offset, offset + 1, ...
     inv_freq: float64 [rot / 2].  A dst may be its own src; otherwise they must not overlap."""
-    n = len(segments)
     x0 = segments[0][0]
     B, T, _, d = x0.shape
-    dev, dt = x0.device, _dt(x0)
-    ints = []
-    for src, dst, _ in segments:
-        if not (src.is_cuda and src.device == dev and dst.device == dev):
+    dev, dtype = x0.device, x0.dtype
+    ptrs, strides, heads = [], [], []
+    for src, dst, rotate in segments:
+        shape = src.shape
+        if src.device != dev or dst.device != dev:
             raise ValueError("tensors must live on one CUDA device")
-        if src.dtype != x0.dtype or dst.dtype != x0.dtype or src.shape != dst.shape or src.dim() != 4 or src.shape[:2] != x0.shape[:2] or src.shape[3] != d:
+        if src.dtype != dtype or dst.dtype != dtype or shape != dst.shape or len(shape) != 4 or shape[0] != B or shape[1] != T or shape[3] != d:
             raise ValueError("segments must agree in dtype, batch, tokens and d")
-        if d > 1 and (src.stride(3) != 1 or dst.stride(3) != 1):
+        a, b = src.stride(), dst.stride()
+        if d > 1 and (a[3] != 1 or b[3] != 1):
             raise ValueError("the values of a head must be adjacent")
-        ints += [*src.stride()[:3], *dst.stride()[:3]]
-    if not (inv_freq.is_cuda and inv_freq.device == dev and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+        ptrs.append((src.data_ptr(), dst.data_ptr()))
+        strides += [a[0], a[1], a[2], b[0], b[1], b[2]]
+        heads.append((shape[2], 1 if rotate else 0))
+    rotary_raw(ptrs, strides, heads, dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse)
+
+
+def rotary_raw(ptrs, strides, heads, dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse):
+    """The launch behind rotary(): ptrs [(src, dst)], strides six integers a segment (batch, token, head of src and dst), heads [(count, rotate)]
+    of segments that the caller has checked; inv_freq and positions are checked here."""
+    n = len(ptrs)
+    if dev.type != "cuda":
+        raise ValueError("tensors must live on a CUDA device")
+    if inv_freq.device != dev or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 vector on the tensors' device")
     pos_ptr, i64, pb, pt = None, 0, 0, 0
     if positions is not None:
         if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
             raise ValueError("positions must be int32 or int64 on the tensors' device")
-        if tuple(positions.shape) == (T,):
+        if positions.shape == (T,):
             pt = positions.stride(0)
-        elif tuple(positions.shape) == (B, T):
+        elif positions.shape == (B, T):
             pb, pt = positions.stride()
         else:
             raise ValueError(f"positions must have shape ({T},) or ({B}, {T}), not {tuple(positions.shape)}")
-        pos_ptr, i64 = _ptr(positions), int(positions.dtype == torch.int64)
-    srcs = (C.c_void_p * n)(*[s.data_ptr() for s, _, _ in segments])
-    dsts = (C.c_void_p * n)(*[t.data_ptr() for _, t, _ in segments])
+        pos_ptr, i64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
+    if dtype not in _LIST_DT:
+        raise ValueError(f"dtype {dtype} not supported (bf16 or fp32)")
     if B * T == 0:
         return
+    longs = array("q", [a for a, _ in ptrs] + [b for _, b in ptrs] + strides)
+    ints = array("i", [h for h, _ in heads] + [r for _, r in heads])
+    at, it = longs.buffer_info()[0], ints.buffer_info()[0]
     with _on(dev):
-        rc = _lib.load().quartet_rotary(n, srcs, dsts, (C.c_int64 * (6 * n))(*ints), (C.c_int32 * n)(*[s.shape[2] for s, _, _ in segments]),
-                                        (C.c_int32 * n)(*[int(bool(r)) for _, _, r in segments]), dt, B, T, d, 2 * inv_freq.numel(), int(bool(interleaved)),
-                                        pos_ptr, i64, pb, pt, int(offset), _ptr(inv_freq), float(scale), int(bool(inverse)), _stream())
-    _lib.check(rc, "quartet_rotary")
+        rc = _lib.load().quartet_rotary(n, at, at + 8 * n, at + 16 * n, it, it + 4 * n, _LIST_DT[dtype], B, T, d, 2 * inv_freq.numel(),
+                                        1 if interleaved else 0, pos_ptr, i64, pb, pt, offset, inv_freq.data_ptr(), scale, 1 if inverse else 0, _stream())
+    if rc:
+        _lib.check(rc, "quartet_rotary")
 
 
 # ------------------------------------------------------------------------------------------------
 # norm over many tensors, and clipping by it
 # ------------------------------------------------------------------------------------------------
 NORM_PARTIALS = 1024
-_LIST_DT = {torch.bfloat16: BF16, torch.float32: F32}
 
 
 def _dense(t) -> bool:
@@ -573,11 +590,15 @@ def _dense(t) -> bool:
 
 
 def _tensor_list(ts, dev, what):
-    for t in ts:
-        if t.device != dev or t.dtype not in _LIST_DT or not _dense(t):
-            raise ValueError(f"{what} must be dense bf16 or fp32 tensors on one CUDA device")
-    n = len(ts)
-    return (C.c_void_p * n)(*[t.data_ptr() for t in ts]), (C.c_int64 * n)(*[t.numel() for t in ts]), (C.c_int32 * n)(*[_LIST_DT[t.dtype] for t in ts])
+    """Host arrays (addresses, element counts, dtypes) of the tensors."""
+    dts = [_LIST_DT.get(t.dtype, -1) for t in ts]
+    if dev.type != "cuda" or -1 in dts or any([t.device != dev for t in ts]) or not all([t.is_contiguous() or _dense(t) for t in ts]):
+        raise ValueError(f"{what} must be dense bf16 or fp32 tensors on one CUDA device")
+    return array("q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]), array("i", dts)
+
+
+def _at(a) -> int:
+    return a.buffer_info()[0]
 
 
 def _norm_kind(norm_type) -> int:
@@ -592,14 +613,14 @@ def grad_norm(tensors, norm_type=2.0, total=False):
     """Norm over all elements of the tensors (bf16 / fp32, mixed): fp32 scalar on their device.  total=True returns instead what ranks that hold
     different tensors combine: the float64 sum of squares, shape [1] (for the maximum norm, the maximum)."""
     tensors, kind = list(tensors), _norm_kind(norm_type)
-    if not tensors or not tensors[0].is_cuda:
-        raise ValueError("need at least one tensor, on a CUDA device")
+    if not tensors:
+        raise ValueError("need at least one tensor")
     dev = tensors[0].device
     ptrs, numels, dts = _tensor_list(tensors, dev, "tensors")
     work = torch.empty(NORM_PARTIALS + 1, dtype=torch.float64, device=dev)
     out = work[NORM_PARTIALS:] if total else torch.empty((), dtype=torch.float32, device=dev)
     with _on(dev):
-        rc = _lib.load().quartet_grad_norm(len(tensors), ptrs, numels, dts, kind, _ptr(work), _ptr(out) if total else None, None if total else _ptr(out),
+        rc = _lib.load().quartet_grad_norm(len(tensors), _at(ptrs), _at(numels), _at(dts), kind, _ptr(work), _ptr(out) if total else None, None if total else _ptr(out),
                                            _stream())
     _lib.check(rc, "quartet_grad_norm")
     return out
@@ -610,15 +631,15 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
     returns the norm before (fp32 scalar on the device; nothing waits for it).  total: a float64 [1] as grad_norm(..., total=True) returns it, e.g.
     summed over ranks, to use in place of the tensors' own."""
     tensors, kind = list(tensors), _norm_kind(norm_type)
-    if not tensors or not tensors[0].is_cuda:
-        raise ValueError("need at least one tensor, on a CUDA device")
+    if not tensors:
+        raise ValueError("need at least one tensor")
     dev = tensors[0].device
     ptrs, numels, dts = _tensor_list(tensors, dev, "tensors")
     optrs, odts = ptrs, dts
     if out is not None:
         out = list(out)
-        if len(out) != len(tensors) or any(o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))
-                                           for o, t in zip(out, tensors)):
+        if len(out) != len(tensors) or any([o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))
+                                            for o, t in zip(out, tensors)]):
             raise ValueError("out must hold a tensor of the same shape and strides for each of the tensors")
         optrs, _, odts = _tensor_list(out, dev, "out")
     if total is not None and not (total.is_cuda and total.device == dev and total.dtype == torch.float64 and total.numel() == 1):
@@ -626,7 +647,7 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
     work = torch.empty(NORM_PARTIALS, dtype=torch.float64, device=dev) if total is None else None
     norm = torch.empty((), dtype=torch.float32, device=dev)
     with _on(dev):
-        rc = _lib.load().quartet_clip_grads(len(tensors), ptrs, optrs, numels, dts, odts, kind, float(max_norm), _ptr(total), _ptr(work), _ptr(norm), _stream())
+        rc = _lib.load().quartet_clip_grads(len(tensors), _at(ptrs), _at(optrs), _at(numels), _at(dts), _at(odts), kind, float(max_norm), _ptr(total), _ptr(work), _ptr(norm), _stream())
     _lib.check(rc, "quartet_clip_grads")
     return norm
 

@@ -12,7 +12,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import ops, torch_ops  # noqa: F401  (torch_ops registers the operators that a compiled model calls)
 from .producers import _out_dtype
@@ -31,8 +30,9 @@ class _Fp8LinearFn(torch.autograd.Function):
         return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, e):
+        if torch.is_grad_enabled():
+            raise RuntimeError("fp8_linear is not differentiable twice")
         xtc, xts, wtc, wts = ctx.saved_tensors
         grad_dtype, x_dtype, w_dtype = ctx.dtypes
         need_dx, need_dw = ctx.needs_input_grad[:2]

@@ -12,7 +12,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops, torch_ops
 
@@ -75,26 +74,36 @@ def _adjacent(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _turn(xs, inv_freq, positions, offset, interleaved, scale, inverse):
+    xs = [_adjacent(x) for x in xs]
+    outs = [torch.empty_like(x) for x in xs]
+    ops.rotary([(x, y, True) for x, y in zip(xs, outs)], inv_freq, positions, offset, interleaved, scale, inverse)
+    return outs
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, inv_freq, positions, offset, interleaved, scale):
+    def forward(ctx, q, k, inv_freq, positions, offset, interleaved, scale, inverse):
         ctx.save_for_backward(inv_freq, positions)
-        ctx.args = (offset, interleaved, scale)
-        xs = [_adjacent(x) for x in (q, k) if x is not None]
-        outs = [torch.empty_like(x) for x in xs]
-        ops.rotary([(x, y, True) for x, y in zip(xs, outs)], inv_freq, positions, *ctx.args)
-        return outs[0], (outs[1] if k is not None else None)
+        ctx.args = (offset, interleaved, scale, inverse)
+        ctx.set_materialize_grads(False)
+        if k is None:
+            return _turn((q,), inv_freq, positions, *ctx.args)[0], None
+        return tuple(_turn((q, k), inv_freq, positions, *ctx.args))
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
+    def backward(ctx, dq, dk):
         inv_freq, positions = ctx.saved_tensors
-        gs = [_adjacent(g) for g, need in zip(grads, ctx.needs_input_grad) if need and g is not None]
-        outs = [torch.empty_like(g) for g in gs]
-        if gs:
-            ops.rotary([(g, y, True) for g, y in zip(gs, outs)], inv_freq, positions, *ctx.args, inverse=True)
-        it = iter(outs)
-        return (*[next(it) if need and g is not None else None for g, need in zip(grads, ctx.needs_input_grad)], None, None, None, None, None)
+        offset, interleaved, scale, inverse = ctx.args
+        need_q, need_k = dq is not None and ctx.needs_input_grad[0], dk is not None and ctx.needs_input_grad[1]
+        gs = ([dq] if need_q else []) + ([dk] if need_k else [])
+        if not gs:
+            return (None,) * 8
+        if torch.is_grad_enabled():  # create_graph: the gradient is a rotation too
+            outs = _Rotary.apply(gs[0], gs[1] if len(gs) == 2 else None, inv_freq, positions, offset, interleaved, scale, not inverse)
+        else:
+            outs = _turn(gs, inv_freq, positions, offset, interleaved, scale, not inverse)
+        return outs[0] if need_q else None, outs[-1 if len(gs) == 2 else 0] if need_k else None, None, None, None, None, None, None
 
 
 def _check_heads(x, what):
@@ -112,23 +121,26 @@ def apply_rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=True, 
         turn = torch.ops.quartet_b200.rotary
         return (turn(q, inv_freq, positions, offset, interleaved, scale, False),
                 None if k is None else turn(k, inv_freq, positions, offset, interleaved, scale, False))
-    return _Rotary.apply(q, k, inv_freq, positions, offset, interleaved, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, inv_freq, positions, offset, interleaved, scale, False)
+    if k is None:
+        return _turn((q,), inv_freq, positions, offset, interleaved, scale, False)[0], None
+    return tuple(_turn((q, k), inv_freq, positions, offset, interleaved, scale, False))
 
 
 class _RotaryQKV(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major):
         ctx.save_for_backward(inv_freq, positions)
-        ctx.args, ctx.head_major = (offset, interleaved, scale), head_major
+        ctx.args = (offset, interleaved, scale, head_major)
         return torch_ops.split_heads(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk, dv):
         inv_freq, positions = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            return (None,) * 9
-        return (torch_ops.join_heads(dq, dk, dv, ctx.head_major, inv_freq, positions, *ctx.args),) + (None,) * 8
+        if torch.is_grad_enabled():
+            raise RuntimeError("rotary_qkv is not differentiable twice: use apply_rotary under create_graph")
+        return torch_ops.join_heads(dq, dk, dv, inv_freq, positions, *ctx.args), None, None, None, None, None, None, None, None
 
 
 def rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions=None, *, offset=0, interleaved=True, scale=1.0, head_major=True):
@@ -138,4 +150,6 @@ def rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions=None, *, offset=0, in
         raise ValueError("qkv must be [batch, tokens, (n_head + 2 n_kv_head) * d]")
     if torch.compiler.is_compiling():
         return torch.ops.quartet_b200.rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
-    return _RotaryQKV.apply(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _RotaryQKV.apply(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
+    return torch_ops.split_heads(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)

@@ -426,34 +426,43 @@ torch.library.register_autograd("quartet_b200::swiglu_linear_fwd", _swiglu_linea
 # ------------------------------------------------------------------------------------------------
 def split_heads(qkv: Tensor, n_head: int, n_kv_head: int, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
                 head_major: bool) -> Tuple[Tensor, Tensor, Tensor]:
-    """Packed projection -> q, k (turned) and v in one launch."""
-    qkv = qkv if qkv.stride(-1) == 1 else qkv.contiguous()
+    """Packed projection -> q, k (turned) and v in one launch.  Addresses and strides are worked out here: a view of torch's costs more
+    than the launch."""
+    if qkv.stride(2) != 1:
+        qkv = qkv.contiguous()
     b, t, w = qkv.shape
     d = w // (n_head + 2 * n_kv_head)
-    outs, segments, at = [], [], 0
-    for i, h in enumerate((n_head, n_kv_head, n_kv_head)):
-        y = qkv.new_empty((b, h, t, d) if head_major else (b, t, h, d))
-        src = qkv[..., at:at + h * d].unflatten(-1, (h, d))
-        outs.append(y)
-        segments.append((src, y.transpose(1, 2) if head_major else y, i < 2))
-        at += h * d
-    ops.rotary(segments, inv_freq, positions, offset, interleaved, scale)
-    return outs[0], outs[1], outs[2]
+    sb, st, _ = qkv.stride()
+    q = qkv.new_empty((b, n_head, t, d) if head_major else (b, t, n_head, d))
+    k, v = (qkv.new_empty((b, n_kv_head, t, d) if head_major else (b, t, n_kv_head, d)) for _ in range(2))
+    src, es = qkv.data_ptr(), qkv.element_size()
+    ptrs = [(src, q.data_ptr()), (src + n_head * d * es, k.data_ptr()), (src + (n_head + n_kv_head) * d * es, v.data_ptr())]
+    strides = []
+    for h in (n_head, n_kv_head, n_kv_head):
+        strides += [sb, st, d, h * t * d, d, t * d] if head_major else [sb, st, d, t * h * d, h * d, d]
+    ops.rotary_raw(ptrs, strides, [(n_head, 1), (n_kv_head, 1), (n_kv_head, 0)], qkv.device, qkv.dtype, b, t, d, inv_freq, positions, offset, interleaved, scale,
+                   False)
+    return q, k, v
 
 
-def join_heads(dq: Tensor, dk: Tensor, dv: Tensor, head_major: bool, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool,
-               scale: float) -> Tensor:
+def join_heads(dq: Tensor, dk: Tensor, dv: Tensor, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
+               head_major: bool) -> Tensor:
     """The gradient of split_heads: gradients of q, k, v (any strides) -> the packed one."""
-    gs = [g.transpose(1, 2) if head_major else g for g in (dq, dk, dv)]
-    b, t, _, d = gs[0].shape
-    out = dq.new_empty(b, t, sum(g.shape[2] for g in gs) * d)
-    segments, at = [], 0
-    for i, g in enumerate(gs):
-        g = g if g.stride(-1) == 1 or d == 1 else g.contiguous()
-        h = g.shape[2]
-        segments.append((g, out[..., at:at + h * d].unflatten(-1, (h, d)), i < 2))
-        at += h * d
-    ops.rotary(segments, inv_freq, positions, offset, interleaved, scale, inverse=True)
+    gs = [g if g.stride(3) == 1 else g.contiguous() for g in (dq, dk, dv)]
+    ax_t, ax_h = (2, 1) if head_major else (1, 2)
+    b, t, d = dq.shape[0], dq.shape[ax_t], dq.shape[3]
+    heads = [g.shape[ax_h] for g in gs]
+    w = sum(heads) * d
+    out = dq.new_empty((b, t, w))
+    dst, es = out.data_ptr(), out.element_size()
+    ptrs, strides = [], []
+    for g, h in zip(gs, heads):
+        st = g.stride()
+        ptrs.append((g.data_ptr(), dst))
+        strides += [st[0], st[ax_t], st[ax_h], t * w, w, d]
+        dst += h * d * es
+    ops.rotary_raw(ptrs, strides, [(heads[0], 1), (heads[1], 1), (heads[2], 0)], out.device, out.dtype, b, t, d, inv_freq, positions, offset, interleaved, scale,
+                   True)
     return out
 
 
@@ -498,13 +507,13 @@ def _(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, h
 
 
 @torch.library.custom_op("quartet_b200::rotary_qkv_bwd", mutates_args=())
-def rotary_qkv_bwd(dq: Tensor, dk: Tensor, dv: Tensor, head_major: bool, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool,
-                   scale: float) -> Tensor:
-    return join_heads(dq, dk, dv, head_major, inv_freq, positions, offset, interleaved, scale)
+def rotary_qkv_bwd(dq: Tensor, dk: Tensor, dv: Tensor, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
+                   head_major: bool) -> Tensor:
+    return join_heads(dq, dk, dv, inv_freq, positions, offset, interleaved, scale, head_major)
 
 
 @rotary_qkv_bwd.register_fake
-def _(dq, dk, dv, head_major, inv_freq, positions, offset, interleaved, scale):
+def _(dq, dk, dv, inv_freq, positions, offset, interleaved, scale, head_major):
     h, t = (1, 2) if head_major else (2, 1)
     return dq.new_empty(dq.shape[0], dq.shape[t], (dq.shape[h] + dk.shape[h] + dv.shape[h]) * dq.shape[3])
 
@@ -512,12 +521,12 @@ def _(dq, dk, dv, head_major, inv_freq, positions, offset, interleaved, scale):
 def _rotary_qkv_setup(ctx, inputs, output):
     _, _, _, inv_freq, positions, offset, interleaved, scale, head_major = inputs
     ctx.save_for_backward(inv_freq, positions)
-    ctx.args, ctx.head_major = (offset, interleaved, scale), head_major
+    ctx.args = (offset, interleaved, scale, head_major)
 
 
 def _rotary_qkv_backward(ctx, dq, dk, dv):
     inv_freq, positions = ctx.saved_tensors
-    return (torch.ops.quartet_b200.rotary_qkv_bwd(dq, dk, dv, ctx.head_major, inv_freq, positions, *ctx.args),) + (None,) * 8
+    return (torch.ops.quartet_b200.rotary_qkv_bwd(dq, dk, dv, inv_freq, positions, *ctx.args),) + (None,) * 8
 
 
 torch.library.register_autograd("quartet_b200::rotary_qkv", _rotary_qkv_backward, setup_context=_rotary_qkv_setup)

@@ -182,3 +182,16 @@ def test_refusals(R):
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_gradient_of_the_gradient(R):
+    """apply_rotary's gradient is itself a rotation, so a second derivative goes through; the packed form refuses one."""
+    inv, _ = R.rotary_frequencies(16, device="cuda")
+    q = torch.randn(1, 4, 2, 16, device="cuda", requires_grad=True)
+    e = torch.randn(1, 4, 2, 16, device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(R.apply_rotary(q, None, inv, scale=1.5)[0], (q,), e, create_graph=True)
+    (de,) = torch.autograd.grad(dx, (e,), torch.ones_like(dx))
+    check(de, *turn(torch.ones_like(dx), torch.arange(4), inv, 1.5, True))
+    qkv = torch.randn(1, 4, 3 * 16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(R.rotary_qkv(qkv, 1, 1, inv)[0].sum(), (qkv,), create_graph=True)
