@@ -261,6 +261,15 @@ int quartet_gemm_fp8_tn(const uint8_t* a, const uint8_t* a_sf, int a_fmt, const 
                         float alpha, void* d, int d_dtype, int64_t ldd, quartet_stream_t stream);
 
 /*
+ * x [M, K] (bf16 / fp32) through a packed weight, y = alpha * Q(x) . W^T with Q the 1 x 128 quantizer above in e4m3: both steps in one call; up to
+ * eight rows (tokens being generated) in one launch.  w, w_sf: codes [N, pad128(K)] and scales; ldy as above.
+ * workspace: 16-byte aligned device memory of quartet_linear_fp8_workspace_bytes(M, K) bytes, NULL where that is 0.
+ */
+int64_t quartet_linear_fp8_workspace_bytes(int64_t M, int64_t K);
+int quartet_linear_fp8(const void* x, int x_dtype, int64_t M, int64_t K, const uint8_t* w, const uint8_t* w_sf, int w_fmt, int64_t N, float alpha,
+                       uint8_t* workspace, void* y, int y_dtype, int64_t ldy, quartet_stream_t stream);
+
+/*
  * Rotary positions (applied to q and k in LlamaAttention, src/models/llama.py:117-158): in every head, pair i of the first `rot` of d values turns
  * by pos * inv_freq[i], the result times `scale`; the other values are copied.  interleaved 1: pairs (2 i, 2 i + 1), the reference's
  * layout; 0: pairs (i, i + rot / 2).  inverse 1: by the negative angle (the gradient).

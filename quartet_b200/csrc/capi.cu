@@ -145,6 +145,7 @@ extern "C" __attribute__((visibility("default"))) int quartet_device_status(int3
     if ((rc = status_probe(status))) return rc;
     if ((rc = status_producer(status))) return rc;
     if ((rc = status_gemm_fp8(status))) return rc;
+    if ((rc = status_gemv_fp8(status))) return rc;
     return QUARTET_OK;
 }
 

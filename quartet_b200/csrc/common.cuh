@@ -34,6 +34,7 @@ int status_aux(int32_t* out);
 int status_probe(int32_t* out);
 int status_producer(int32_t* out);
 int status_gemm_fp8(int32_t* out);
+int status_gemv_fp8(int32_t* out);
 
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per kernel instantiation, thread and device instead of
 // before every launch.  `state` is a thread_local int of the calling (template) function, initialised to -1.

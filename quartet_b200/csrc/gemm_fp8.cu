@@ -10,25 +10,14 @@
 // gemm_fp8_split_kernel: few rows of A, or a small result.  The roles are swapped -- 128 rows of B are the instruction's M
 // and up to 128 rows of A its N -- so that a single token still feeds every row of the tensor core with one weight row, and
 // the contraction is split over the CTAs of a cluster, which add their fp32 partial results in rank order through
-// distributed shared memory: no workspace, no atomics, the same bits every time.
+// distributed shared memory: no workspace, no atomics, the same bits every time.  (Up to eight rows go to gemv_fp8.cu.)
 #include "common.cuh"
+#include "gemm_fp8.cuh"
 #include "tcgen05.cuh"
 
 #include <cuda_bf16.h>
 
 namespace quartet {
-
-struct Fp8GemmParams {
-    const uint8_t* a_sf;
-    const uint8_t* b_sf;
-    int64_t M, N;
-    int64_t ldd;
-    int k_chunks;        // K / 128
-    int a_e5m2, b_e5m2;
-    float alpha;
-    void* d;
-    int d_f32;
-};
 
 // Instruction descriptor, kind::mxf8f6f4, UE8M0 scales, both operands K-major.
 __device__ __forceinline__ uint32_t make_idesc_fp8(int m, int n, int a_e5m2, int b_e5m2, uint32_t sf_id) {
@@ -51,16 +40,6 @@ __device__ __forceinline__ void tc_mma_mxf8(uint32_t d_tmem, uint64_t adesc, uin
         : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
         : "memory");
 }
-// One 512-byte scale block from shared memory to four tensor-memory columns, replicated into the four lane quadrants.  Ordered
-// with the MMAs the same thread issues.
-__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(128 >> 4) << 32;    // eight 16-byte rows to the next
-    d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-
 // ---------------------------------------------------------------------------
 // swapped roles, contraction split over a cluster
 // ---------------------------------------------------------------------------
@@ -68,20 +47,20 @@ template <int BT>  // rows of A (tokens) a CTA takes
 struct SplitCfg {
     static constexpr int W_BYTES = 128 * 128;
     static constexpr int X_BYTES = BT * 128;
-    static constexpr int STAGES = BT == 128 ? 6 : 8;
+    static constexpr int STAGES = BT == 128 ? 3 : BT == 64 ? 4 : 5;   // two CTAs on an SM: one's start and end run under the other's copies
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 1024;
     static constexpr int SF_COL0 = BT;
-    static constexpr int TMEM_COLS = BT == 128 ? 256 : 128;   // BT accumulator columns and eight scale columns a stage
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 256;
+    static constexpr int TMEM_COLS = BT == 128 ? 256 : 128;           // BT accumulator columns and eight scale columns a stage
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 512;
     static_assert(SF_COL0 + STAGES * 8 <= TMEM_COLS, "tensor memory capacity");
     static_assert(STAGES * (W_BYTES + X_BYTES) >= BT * 128 * 4, "the partial result reuses the operand stages");
-    static_assert(SMEM <= 232448, "shared memory capacity");
+    static_assert(SMEM <= 113 * 1024, "two CTAs share an SM");
 };
 
-constexpr int SPLIT_THREADS = 128;
+constexpr int SPLIT_THREADS = 256, SPLIT_MAX = 8;  // warps 0, 2, 3 issue copies (weight, A, scales), 1 the MMAs; 4-7 feed scales, then drain
 
 template <int BT>
-__global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+__global__ void __launch_bounds__(SPLIT_THREADS, 2) gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                                                                          const Fp8GemmParams p, const int splits) {
     using C = SplitCfg<BT>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -95,7 +74,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
     uint8_t* s_sf = s_x + C::STAGES * C::X_BYTES;
     uint64_t* full = reinterpret_cast<uint64_t*>(s_sf + C::STAGES * 1024);
     uint64_t* empty = full + C::STAGES;
-    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* sf_land = empty + C::STAGES;
+    uint64_t* sf_full = sf_land + C::STAGES;
+    uint64_t* acc_full = sf_full + C::STAGES;
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_full + 1);
     volatile int* dead = reinterpret_cast<volatile int*>(s_tmem + 1);
 
@@ -106,8 +87,10 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 2);
             mbar_init(&empty[i], 1);
+            mbar_init(&sf_land[i], 1);
+            mbar_init(&sf_full[i], 4);
         }
         mbar_init(acc_full, 1);
         *dead = 0;
@@ -126,28 +109,14 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
     pdl_launch_dependents();
     pdl_wait();
 
-    if (warp == 0) {
+    if (warp == 1) {
         if (lane == 0) {
             uint32_t s = 0, ph = 0;
             for (int c = c0; c < c1; ++c) {
-                if (!gemm_wait(&empty[s], ph ^ 1, WAIT_GEMM_EMPTY, dead)) break;
-                mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
-                tma_load_2d(s_w + s * C::W_BYTES, &tm_w, c * 128, n_blk * 128, &full[s]);
-                tma_load_2d(s_x + s * C::X_BYTES, &tm_x, c * 128, t_blk * BT, &full[s]);
-                bulk_load(s_sf + s * 1024, p.b_sf + ((int64_t)n_blk * p.k_chunks + c) * 512, 512, &full[s]);
-                bulk_load(s_sf + s * 1024 + 512, p.a_sf + ((int64_t)(t_blk * BT / 128) * p.k_chunks + c) * 512, 512, &full[s]);
-                if (++s == C::STAGES) s = 0, ph ^= 1;
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t s = 0, ph = 0;
-            for (int c = c0; c < c1; ++c) {
+                if (!gemm_wait(&sf_full[s], ph, WAIT_GEMM_SF, dead)) break;
                 if (!gemm_wait(&full[s], ph, WAIT_GEMM_FULL, dead)) break;
                 tc_fence_after();
                 const uint32_t sf = tmem + C::SF_COL0 + s * 8;
-                tc_cp_scales(sf, smem_u32(s_sf + s * 1024));
-                tc_cp_scales(sf + 4, smem_u32(s_sf + s * 1024 + 512));
                 const uint64_t wd = make_desc_sw128(smem_u32(s_w + s * C::W_BYTES)), xd = make_desc_sw128(smem_u32(s_x + s * C::X_BYTES));
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j)  // 32 values a step, one scale byte each
@@ -158,22 +127,62 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
             }
             tc_commit(acc_full);
         }
+    } else if (warp < 4) {
+        // three threads in three warps: one thread starts a copy only every few hundred cycles
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            for (int c = c0; c < c1; ++c) {
+                if (!gemm_wait(&empty[s], ph ^ 1, WAIT_GEMM_EMPTY, dead)) break;
+                if (warp == 0) {
+                    mbar_arrive_expect_tx(&full[s], C::W_BYTES);
+                    tma_load_2d(s_w + s * C::W_BYTES, &tm_w, c * 128, n_blk * 128, &full[s]);
+                } else if (warp == 2) {
+                    mbar_arrive_expect_tx(&full[s], C::X_BYTES);
+                    tma_load_2d(s_x + s * C::X_BYTES, &tm_x, c * 128, t_blk * BT, &full[s]);
+                } else {
+                    mbar_arrive_expect_tx(&sf_land[s], 1024);
+                    bulk_load(s_sf + s * 1024, p.b_sf + ((int64_t)n_blk * p.k_chunks + c) * 512, 512, &sf_land[s]);
+                    bulk_load(s_sf + s * 1024 + 512, p.a_sf + ((int64_t)(t_blk * BT / 128) * p.k_chunks + c) * 512, 512, &sf_land[s]);
+                }
+                if (++s == C::STAGES) s = 0, ph ^= 1;
+            }
+        }
+    } else {
+        // Scales go to tensor memory through registers, a warp per lane quadrant.  (A copy issued among the MMAs orders itself with them:
+        // the chain copy -> MMA -> copy took 745 cycles a stage, whatever the number of stages or of issuing threads.)
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t s = 0, ph = 0;
+        for (int c = c0; c < c1; ++c) {
+            if (!gemm_wait(&sf_land[s], ph, WAIT_GEMM_FULL, dead)) break;
+            const uint4 w4 = *reinterpret_cast<const uint4*>(s_sf + s * 1024 + lane * 16), x4 = *reinterpret_cast<const uint4*>(s_sf + s * 1024 + 512 + lane * 16);
+            const uint32_t v[8] = {w4.x, w4.y, w4.z, w4.w, x4.x, x4.y, x4.z, x4.w};
+            tc_st8(tmem + lane_base + C::SF_COL0 + s * 8, v);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sf_full[s]);
+            if (++s == C::STAGES) s = 0, ph ^= 1;
+        }
     }
     __syncwarp();
     // ---- partial results [token][weight row] in fp32 over the operand stages: all copies have landed and been read ----
     const bool ok = gemm_wait(acc_full, 0, WAIT_GEMM_ACC_FULL, dead);
     tc_fence_after();
     float* red = reinterpret_cast<float*>(smem);
-    const int row = warp * 32 + lane;
+    const int row = (warp & 3) * 32 + lane;
+    const int64_t t0 = (int64_t)t_blk * BT;
+    const int tokens = (int)(p.M - t0 < BT ? p.M - t0 : BT);
     __syncthreads();
     if (ok) {
+        // two warps per lane quadrant take turns
 #pragma unroll 1
-        for (int cb = 0; cb < BT; cb += 32) {
+        for (int cb = (warp >> 2) * 32; cb < tokens; cb += 64) {
             uint32_t r[32];
-            tc_ld32(tmem + ((uint32_t)(warp * 32) << 16) + cb, r);
+            tc_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + cb, r);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) red[(cb + i) * 128 + row] = __uint_as_float(r[i]);
+            for (int i = 0; i < 32; ++i)
+                if (cb + i < tokens) red[(cb + i) * 128 + row] = __uint_as_float(r[i]);
         }
     }
     tc_fence_before();
@@ -182,22 +191,28 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
     else
         __syncthreads();
     if (ok) {
-        // this CTA adds the partial results of tokens rank, rank + splits, ...; 32 threads a token, four results each
-        const int64_t t0 = (int64_t)t_blk * BT;
-        const int tokens = (int)(p.M - t0 < BT ? p.M - t0 : BT);
-        const int64_t n0 = (int64_t)n_blk * 128 + lane * 4;
-        const uint32_t red_addr = smem_u32(red) + lane * 16;
-        for (int t = rank + warp * splits; t < tokens; t += 4 * splits) {
+        // the tokens' results, four side by side, are dealt out over the threads of the whole cluster
+        const uint32_t red_addr = smem_u32(red);
+        for (int i = rank * SPLIT_THREADS + threadIdx.x; i < tokens * 32; i += splits * SPLIT_THREADS) {
+            const int t = i >> 5;
+            const int64_t n0 = (int64_t)n_blk * 128 + (i & 31) * 4;
+            if (n0 >= p.N) continue;
             float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int s = 0; s < splits; ++s) {
-                const uint32_t at = red_addr + t * 512;
-                float4 q;
-                const uint32_t peer = splits > 1 ? mapa_u32(at, s) : at;
-                if (splits > 1)
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(peer) : "memory");
-                else
-                    q = *reinterpret_cast<const float4*>(red + t * 128 + lane * 4);
-                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            if (splits == 1) {
+                const float4 q = *reinterpret_cast<const float4*>(red + i * 4);
+                v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            } else {
+                float4 q[SPLIT_MAX];
+#pragma unroll
+                for (int s = 0; s < SPLIT_MAX; ++s)
+                    if (s < splits)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(q[s].x), "=f"(q[s].y), "=f"(q[s].z), "=f"(q[s].w)
+                                     : "r"(mapa_u32(red_addr + i * 16, s))
+                                     : "memory");
+#pragma unroll
+                for (int s = 0; s < SPLIT_MAX; ++s)
+                    if (s < splits) v[0] += q[s].x, v[1] += q[s].y, v[2] += q[s].z, v[3] += q[s].w;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] *= p.alpha;
@@ -229,8 +244,22 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1) gemm_fp8_split_kernel(const 
     }
 }
 
+// How many ways the contraction is split: the power of two that gives the busiest SM the least work, a CTA's start and end counted as
+// SPLIT_FIXED chunks of 128.  (us, splits 1 / 2 / 4 / 8: N 12288, K 4096, one row 14.4 / 13.9 / 16.3 / 19.6; N 4096, K 4096 14.0 / 10.6 / 8.5 / 9.2;
+// N 4096, K 11008 30.4 / 18.1 / 12.2 / 11.8; N 32000, K 640 6.0 / 10.3 / 18.0 / 21.4.  Clusters of 3 and 6 lie above their neighbours.)
+constexpr int SPLIT_FIXED = 4;
+static int pick_splits(int64_t tiles, int chunks, int sms) {
+    int best = 1;
+    int64_t cost = INT64_MAX;
+    for (int s = 1; s <= SPLIT_MAX && s <= chunks; s *= 2) {
+        const int64_t per_sm = (tiles * s + sms - 1) / sms, c = per_sm * ((chunks + s - 1) / s + SPLIT_FIXED);
+        if (c < cost) cost = c, best = s;
+    }
+    return best;
+}
+
 template <int BT>
-static int launch_split(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, int splits, cudaStream_t stream) {
+static int launch_split(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t stream) {
     using C = SplitCfg<BT>;
     CUtensorMap tm_w, tm_x;
     int rc = make_tmap_2d(&tm_w, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.N, K, 128, 128, 3);
@@ -239,8 +268,12 @@ static int launch_split(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8
     auto kern = gemm_fp8_split_kernel<BT>;
     static thread_local int smem_set = -1;
     if ((rc = set_max_smem_once(kern, C::SMEM, smem_set))) return rc;
+    int sms = 0;
+    if ((rc = device_sm_count(&sms))) return rc;
+    const int64_t n_tiles = (p.N + 127) / 128, t_tiles = (p.M + BT - 1) / BT;
+    const int splits = pick_splits(n_tiles * t_tiles, p.k_chunks, sms);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.N + 127) / 128 * splits), (unsigned)((p.M + BT - 1) / BT));
+    cfg.gridDim = dim3((unsigned)(n_tiles * splits), (unsigned)t_tiles);
     cfg.blockDim = dim3(SPLIT_THREADS), cfg.dynamicSmemBytes = C::SMEM, cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -593,6 +626,13 @@ static int launch_pair(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8G
 
 QUARTET_DEFINE_STATUS_READER(status_gemm_fp8)
 
+static int product(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t s) {
+    if (gemv_fits(p.M, K)) return gemv_fp8_codes(a, b, p, s);
+    if (p.M >= 256 && p.N >= 256) return launch_pair(a, b, K, p, s);
+    if (p.M > 64) return launch_split<128>(a, b, K, p, s);
+    return p.M > 32 ? launch_split<64>(a, b, K, p, s) : launch_split<32>(a, b, K, p, s);
+}
+
 }  // namespace quartet
 
 using namespace quartet;
@@ -617,7 +657,44 @@ extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_tn(const 
     p.k_chunks = (int)(K / 128);
     p.a_e5m2 = a_fmt, p.b_e5m2 = b_fmt;
     p.alpha = alpha, p.d = d, p.d_f32 = d_dtype == QUARTET_F32;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (M >= 256 && N >= 256) return launch_pair(a, b, K, p, s);
-    return launch_split<128>(a, b, K, p, 1, s);
+    return product(a, b, K, p, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" __attribute__((visibility("default"))) int64_t quartet_linear_fp8_workspace_bytes(int64_t M, int64_t K) {
+    const int64_t pk = (K + 127) / 128 * 128;
+    if (K < 1 || gemv_fits(M, pk)) return 0;
+    return M * pk + quartet_sf_bytes(M, pk);
+}
+
+extern "C" __attribute__((visibility("default"))) int quartet_linear_fp8(const void* x, int x_dtype, int64_t M, int64_t K, const uint8_t* w, const uint8_t* w_sf,
+                                                                         int w_fmt, int64_t N, float alpha, uint8_t* workspace, void* y, int y_dtype, int64_t ldy,
+                                                                         quartet_stream_t stream) {
+    if (!x || !w || !w_sf || !y) return fail(QUARTET_E_NULL, "x, w, w_sf and y must be non-NULL");
+    if (M < 1 || N < 1 || K < 1 || M > 8388480 || N > 8388480 || K > (1 << 30))
+        return fail(QUARTET_E_SHAPE, "need 1 <= M, N <= 8388480 and K >= 1 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
+    // everything is checked before the first of the two steps is launched
+    if (x_dtype != QUARTET_BF16 && x_dtype != QUARTET_F32) return fail(QUARTET_E_ARG, "x_dtype must be 0 (bf16) or 1 (f32)");
+    if (w_fmt != QUARTET_E4M3 && w_fmt != QUARTET_E5M2) return fail(QUARTET_E_ARG, "w_fmt must be 0 (e4m3) or 1 (e5m2)");
+    if (y_dtype != QUARTET_BF16 && y_dtype != QUARTET_F32) return fail(QUARTET_E_ARG, "y_dtype must be 0 or 1");
+    const bool f32 = x_dtype == QUARTET_F32;
+    if (ldy < N || ldy % (y_dtype == QUARTET_F32 ? 4 : 8)) return fail(QUARTET_E_SHAPE, "rows of y must start on 16-byte boundaries and hold N results");
+    if (reinterpret_cast<uintptr_t>(x) & (f32 ? 3u : 1u)) return fail(QUARTET_E_ALIGN, "x must be aligned to its type");
+    if (!aligned16(w) || !aligned16(w_sf) || !aligned16(y) || !aligned16(workspace)) return fail(QUARTET_E_ALIGN, "w, w_sf, y and workspace must be 16-byte aligned");
+    const int64_t pk = (K + 127) / 128 * 128;
+    if (!gemv_fits(M, pk)) {
+        if (!workspace) return fail(QUARTET_E_NULL, "workspace must be non-NULL for %lld rows", (long long)M);
+        uint8_t* sf = workspace + M * pk;  // pk is a multiple of 128, so the scales are aligned like the codes
+        const int rc = quartet_quant_fp8(x, x_dtype, M, K, QUARTET_E4M3, 0, workspace, sf, nullptr, nullptr, stream);
+        return rc ? rc : quartet_gemm_fp8_tn(workspace, sf, QUARTET_E4M3, w, w_sf, w_fmt, M, N, pk, alpha, y, y_dtype, ldy, stream);
+    }
+    int rc = bind_context_of(w);
+    if (rc) return rc;
+    if ((rc = check_device())) return rc;
+    Fp8GemmParams p{};
+    p.b_sf = w_sf;
+    p.M = M, p.N = N, p.ldd = ldy;
+    p.k_chunks = (int)(pk / 128);
+    p.b_e5m2 = w_fmt;
+    p.alpha = alpha, p.d = y, p.d_f32 = y_dtype == QUARTET_F32;
+    return gemv_fp8_values(x, f32, K, w, p, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,291 @@
+// 8-bit block-scaled product for up to eight rows of A (tokens being generated):  D[M, N] = alpha * A[M, K] . B[N, K]^T
+//
+// Every byte of the weight B is used for at most eight results, so the kernel is a stream over B: N K (1 + 1/32) bytes at the memory's rate
+// is its floor.  A CTA of sixteen warps visits blocks of 16 RW rows of B; RW groups of KW = 16 / RW warps each take 16 rows, the
+// warps of a group a share of the contraction each.  A warp owns a ring of tensor copies (16 rows x 128 values and their scales) that
+// runs on into its next block while the present one is reduced, so the stream never pauses, and there is nothing to set up per
+// block: no tensor memory, no cluster.  All SMs take part evenly, which the memory's rate needs: one SM draws at most about 24 bytes a clock from
+// it, however many copies are under way.
+// The products are m16n8k16 in fp16, which holds every 8-bit code: 16 rows of B, converted as they come from shared memory, and the
+// (up to) eight rows of A, converted once.  Sums over 32 values are scaled by their two E8M0 factors in fp32 and added to
+// fp32 sums, which the warps of a group join in a fixed order in shared memory.  (The 8-bit form of the instruction converts both operands
+// inside: 30 us at N 12288, K 4096, one row, against 17.)  Bound by the issue of instructions, about 320 for 2 KB: eight warps take 21 us.
+// us at one row, quantizer included, here / tensor-memory kernel with its quantizer: N 12288, K 4096 17.1 / 16.5; N 4096, K 11008 15.2 / 14.3; N 32000,
+// K 640 8.0 / 8.0, of which a caller pays one launch / two.
+// A comes as codes and scales, or as values that the CTA quantizes into shared memory while its first copies are under way.
+#include "common.cuh"
+#include "gemm_fp8.cuh"
+#include "quant_fp8.cuh"
+
+namespace quartet {
+
+constexpr int GEMV_WARPS = 16, GEMV_THREADS = 32 * GEMV_WARPS, GEMV_STAGES = 3;
+constexpr int GEMV_W_BYTES = 16 * 128, GEMV_SF_BYTES = 256, GEMV_STAGE_BYTES = GEMV_W_BYTES + GEMV_SF_BYTES;
+constexpr int GEMV_RING = GEMV_WARPS * GEMV_STAGES * GEMV_STAGE_BYTES;
+constexpr int GEMV_FIXED = GEMV_RING + 2 * GEMV_WARPS * 128 * 4 + GEMV_WARPS * GEMV_STAGES * 8;
+
+enum { A_CODES = 0, A_BF16 = 1, A_F32 = 2 };
+
+// rows of A in shared memory, in fp16: 32 bytes more than the values, so that four rows' eight-byte reads lie in different banks
+static inline int64_t gemv_pitch(int64_t pk) { return 2 * pk + 32; }
+bool gemv_fits(int64_t M, int64_t pk) { return M <= 8 && M * (gemv_pitch(pk) + pk / 32) <= 96 * 1024; }
+
+__device__ __forceinline__ float e8m0_value(uint32_t b) {
+    return __uint_as_float(b == 255u ? 0x7FC00000u : b == 0u ? 0x00400000u : b << 23);
+}
+
+template <bool E5M2>
+__device__ __forceinline__ uint32_t f16x2_of(uint32_t two) {  // two codes in the low bytes
+    uint32_t h;
+    if constexpr (E5M2)
+        asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    else
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    return h;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct GemvParams {
+    Fp8GemmParams g;
+    const uint8_t* a;       // codes (A_CODES) or values
+    int64_t a_cols;         // values in a row (A_BF16, A_F32)
+    int a_vec;
+    int kw;                 // warps that share a row group's contraction
+    int blocks;             // blocks of 16 * 8 / kw rows
+};
+
+template <int AMODE, bool B_E5M2, bool A_E5M2>
+__global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_constant__ CUtensorMap tm_w, const GemvParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) atomicOr(&g_status, WAIT_GEMM_ALIGN | 0x100);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* s_w = smem + warp * (GEMV_STAGES * GEMV_W_BYTES);
+    uint8_t* s_sf = smem + GEMV_WARPS * GEMV_STAGES * GEMV_W_BYTES + warp * (GEMV_STAGES * GEMV_SF_BYTES);
+    float* s_part = reinterpret_cast<float*>(smem + GEMV_RING);                 // [2][warp][16 rows x 8 tokens]
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_part + 2 * GEMV_WARPS * 128) + warp * GEMV_STAGES;
+    uint8_t* s_a = smem + GEMV_FIXED;
+    const int chunks = p.g.k_chunks, M = (int)p.g.M;
+    const int pitch = chunks * 256 + 32;
+    uint32_t* s_asf = reinterpret_cast<uint32_t*>(s_a + M * pitch);             // [token][chunk], four scale bytes
+    const int kw = p.kw, rw = GEMV_WARPS / kw, kpart = warp % kw, group = warp / kw;
+    const int c0 = chunks * kpart / kw, mine = chunks * (kpart + 1) / kw - c0;
+
+    if (lane == 0) {
+        for (int i = 0; i < GEMV_STAGES; ++i) mbar_init(&full[i], 1);
+        fence_mbar_init();
+        prefetch_tmap(&tm_w);
+    }
+    __syncwarp();
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // the ring's position in this warp's sequence of (block, chunk)
+    int blk = blockIdx.x, ck = 0;
+    auto issue = [&](int s) {  // lane 0
+        const int row0 = (blk * rw + group) * 16;
+        mbar_arrive_expect_tx(&full[s], GEMV_STAGE_BYTES);
+        tma_load_2d(s_w + s * GEMV_W_BYTES, &tm_w, (c0 + ck) * 128, row0, &full[s]);
+        bulk_load(s_sf + s * GEMV_SF_BYTES, p.g.b_sf + ((int64_t)(row0 >> 7) * chunks + c0 + ck) * 512 + (row0 & 31) * 16, GEMV_SF_BYTES, &full[s]);
+    };
+    // blocks whose group lies past the last row are passed over by every lane alike
+    auto skip = [&](int b) { return (int64_t)(b * rw + group) * 16 >= p.g.N; };
+    int ahead = 0;  // copies issued and not yet consumed
+    auto fill = [&](int s) {
+        while (blk < p.blocks && skip(blk)) blk += gridDim.x;
+        if (blk >= p.blocks || mine == 0) return;
+        if (lane == 0) issue(s);
+        ++ahead;
+        if (++ck == mine) ck = 0, blk += gridDim.x;
+    };
+    for (int s = 0; s < GEMV_STAGES; ++s) fill(s);
+
+    // A into shared memory
+    if constexpr (AMODE == A_CODES) {
+        for (int i = tid; i < M * chunks * 8; i += GEMV_THREADS) {
+            const int r = i / (chunks * 8), c = i - r * (chunks * 8);
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.a + (int64_t)r * chunks * 128) + c);
+            uint4* dst = reinterpret_cast<uint4*>(s_a + r * pitch + c * 32);
+            dst[0] = make_uint4(f16x2_of<A_E5M2>(v.x), f16x2_of<A_E5M2>(v.x >> 16), f16x2_of<A_E5M2>(v.y), f16x2_of<A_E5M2>(v.y >> 16));
+            dst[1] = make_uint4(f16x2_of<A_E5M2>(v.z), f16x2_of<A_E5M2>(v.z >> 16), f16x2_of<A_E5M2>(v.w), f16x2_of<A_E5M2>(v.w >> 16));
+        }
+        for (int i = tid; i < M * chunks; i += GEMV_THREADS) {
+            const int r = i / chunks, c = i - r * chunks;
+            s_asf[i] = __ldg(reinterpret_cast<const uint32_t*>(p.g.a_sf + (int64_t)c * 512 + r * 16));
+        }
+    } else {
+        using R = RowPart<AMODE == A_F32>;
+        const int j = tid & 7, n = M * chunks;
+        for (int i0 = 0; i0 < n; i0 += 2 * GEMV_THREADS / 8) {   // two row parts a thread in flight
+            R part[2];
+            int at[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                at[u] = i0 + u * (GEMV_THREADS / 8) + (tid >> 3);
+                const int r = at[u] / chunks;
+                part[u].load(p.a, at[u] < n ? M : 0, p.a_cols, p.a_vec, r, (int64_t)(at[u] - r * chunks) * 128, j);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t sb = fp8_scale_byte(max_over_8(part[u].amax()), 8);
+                if (at[u] >= n) continue;
+                const int r = at[u] / chunks, c = at[u] - r * chunks;
+#pragma unroll
+                for (int q = 0; q < R::N; ++q) {
+                    uint32_t w[R::PER / 4];
+                    part[u].codes(w, q, sb, false);
+                    uint2* dst = reinterpret_cast<uint2*>(s_a + r * pitch + c * 256 + (j + 8 * q) * R::PER * 2);
+#pragma unroll
+                    for (int k = 0; k < R::PER / 4; ++k) dst[k] = make_uint2(f16x2_of<false>(w[k]), f16x2_of<false>(w[k] >> 16));
+                }
+                if (j == 0) s_asf[at[u]] = sb * 0x01010101u;
+            }
+        }
+    }
+    __syncthreads();
+
+    const int g = lane >> 2, q = lane & 3;     // accumulator: rows g, g + 8 of B, tokens 2 q, 2 q + 1
+    const uint8_t* a_row = s_a + (g < M ? g : 0) * pitch + q * 8;
+    const uint32_t* asf0 = s_asf + (2 * q < M ? 2 * q : 0) * chunks;
+    const uint32_t* asf1 = s_asf + (2 * q + 1 < M ? 2 * q + 1 : 0) * chunks;
+    uint32_t s = 0, ph = 0, buf = 0;
+    bool dead = false;                         // a wait gave up: this warp only keeps the barriers
+    for (int b = blockIdx.x; b < p.blocks; b += gridDim.x, buf ^= 1) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        const int row0 = (b * rw + group) * 16;
+        if (!dead && !skip(b)) {
+            const int seg = (row0 >> 5) & 3;
+            for (int c = 0; c < mine; ++c) {
+                if (!mbar_wait(&full[s], ph, WAIT_GEMM_FULL)) {
+                    dead = true;
+                    break;
+                }
+                --ahead;
+                const uint8_t* sfw = s_sf + s * GEMV_SF_BYTES + seg * 4;
+                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(sfw + g * 16), w1 = *reinterpret_cast<const uint32_t*>(sfw + (g + 8) * 16);
+                const uint32_t x0 = asf0[c0 + c], x1 = asf1[c0 + c];
+                const uint32_t base = smem_u32(s_w + s * GEMV_W_BYTES);
+                // ldmatrix: lanes 0-7 rows 0-7, 8-15 rows 8-15 of the first 16 bytes, 16-31 the same of the second
+                const int mrow = lane & 15, half = lane >> 4;
+                const uint8_t* av = a_row + (c0 + c) * 256;
+                float cc[4][4] = {};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t f[4];
+                    const uint32_t addr = base + mrow * 128 + (((2 * k + half) ^ (mrow & 7)) << 4);
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+                                 : "r"(addr)
+                                 : "memory");
+                    // a thread's four neighbouring values of a row stand for the instruction's columns 2 q, 2 q + 1, 2 q + 8, 2 q + 9, and so do A's
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint2 xv = *reinterpret_cast<const uint2*>(av + k * 64 + h * 32);
+                        if (g >= M) xv = make_uint2(0u, 0u);
+                        mma_f16(cc[k], f16x2_of<B_E5M2>(f[2 * h]), f16x2_of<B_E5M2>(f[2 * h + 1]), f16x2_of<B_E5M2>(f[2 * h] >> 16),
+                                f16x2_of<B_E5M2>(f[2 * h + 1] >> 16), xv.x, xv.y);
+                    }
+                }
+                __syncwarp();
+                fill((int)s);  // the stage is in registers: its next copy may start
+                if (++s == GEMV_STAGES) s = 0, ph ^= 1;
+                const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0);
+                if (__all_sync(0xFFFFFFFFu, block)) {  // one scale for the whole chunk, as this library's quantizers write them
+                    const float sw0 = e8m0_value(w0 & 255u), sw1 = e8m0_value(w1 & 255u), sx0 = e8m0_value(x0 & 255u), sx1 = e8m0_value(x1 & 255u);
+                    acc[0] = fmaf(((cc[0][0] + cc[1][0]) + (cc[2][0] + cc[3][0])) * sw0, sx0, acc[0]);
+                    acc[1] = fmaf(((cc[0][1] + cc[1][1]) + (cc[2][1] + cc[3][1])) * sw0, sx1, acc[1]);
+                    acc[2] = fmaf(((cc[0][2] + cc[1][2]) + (cc[2][2] + cc[3][2])) * sw1, sx0, acc[2]);
+                    acc[3] = fmaf(((cc[0][3] + cc[1][3]) + (cc[2][3] + cc[3][3])) * sw1, sx1, acc[3]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float sw0 = e8m0_value((w0 >> (8 * k)) & 255u), sw1 = e8m0_value((w1 >> (8 * k)) & 255u);
+                        const float sx0 = e8m0_value((x0 >> (8 * k)) & 255u), sx1 = e8m0_value((x1 >> (8 * k)) & 255u);
+                        acc[0] = fmaf(cc[k][0] * sw0, sx0, acc[0]);
+                        acc[1] = fmaf(cc[k][1] * sw0, sx1, acc[1]);
+                        acc[2] = fmaf(cc[k][2] * sw1, sx0, acc[2]);
+                        acc[3] = fmaf(cc[k][3] * sw1, sx1, acc[3]);
+                    }
+                }
+            }
+        }
+        float* part = s_part + (buf * GEMV_WARPS + warp) * 128;   // [token][row]
+        part[(2 * q) * 16 + g] = acc[0], part[(2 * q + 1) * 16 + g] = acc[1];
+        part[(2 * q) * 16 + g + 8] = acc[2], part[(2 * q + 1) * 16 + g + 8] = acc[3];
+        __syncthreads();  // one barrier a block: the partial sums alternate between two buffers
+        for (int i = tid; i < rw * 16 * M; i += GEMV_THREADS) {
+            const int row = i % (rw * 16), tok = i / (rw * 16), gr = row >> 4;
+            const int64_t n = (int64_t)b * rw * 16 + row;
+            float v = 0.f;
+            for (int k = 0; k < kw; ++k) v += s_part[(buf * GEMV_WARPS + gr * kw + k) * 128 + tok * 16 + (row & 15)];
+            v *= p.g.alpha;
+            if (n < p.g.N) {
+                if (p.g.d_f32)
+                    static_cast<float*>(p.g.d)[tok * p.g.ldd + n] = v;
+                else
+                    static_cast<__nv_bfloat16*>(p.g.d)[tok * p.g.ldd + n] = __float2bfloat16_rn(v);
+            }
+        }
+    }
+    // after a wait that gave up, copies may still be in flight: they land before shared memory is released
+    for (int i = 0; i < GEMV_STAGES && ahead > 0; ++i, --ahead) {
+        mbar_wait(&full[s], ph, WAIT_GEMM_FULL);
+        if (++s == GEMV_STAGES) s = 0, ph ^= 1;
+    }
+}
+
+// KW, the warps that share a row's contraction: the number for which the SM with the most blocks has the least to do, a block's reduction
+// counted as one more chunk.
+static int gemv_pick_kw(int64_t N, int chunks, int sms) {
+    int best = 1;
+    int64_t cost = INT64_MAX;
+    for (int kw = 1; kw <= GEMV_WARPS && kw <= chunks; kw *= 2) {
+        const int64_t rows = 16 * (GEMV_WARPS / kw), blocks = (N + rows - 1) / rows;
+        const int64_t c = ((blocks + sms - 1) / sms) * ((chunks + kw - 1) / kw + 1);
+        if (c <= cost) cost = c, best = kw;
+    }
+    return best;
+}
+
+template <int AMODE, bool B_E5M2, bool A_E5M2>
+static int launch_gemv(const uint8_t* b, GemvParams p, cudaStream_t stream) {
+    const int64_t K = (int64_t)p.g.k_chunks * 128;
+    CUtensorMap tm_w;
+    int rc = make_tmap_2d(&tm_w, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.g.N, K, 128, 16, 3);
+    if (rc) return rc;
+    int sms = 0;
+    if ((rc = device_sm_count(&sms))) return rc;
+    p.kw = gemv_pick_kw(p.g.N, p.g.k_chunks, sms);
+    const int rows = 16 * (GEMV_WARPS / p.kw);
+    p.blocks = (int)((p.g.N + rows - 1) / rows);
+    const int smem = GEMV_FIXED + (int)(p.g.M * (gemv_pitch(K) + K / 32));
+    auto kern = gemv_fp8_kernel<AMODE, B_E5M2, A_E5M2>;
+    static thread_local int smem_set = -1;
+    if ((rc = set_max_smem_once(kern, GEMV_FIXED + 96 * 1024, smem_set))) return rc;
+    const int grid = p.blocks < sms ? p.blocks : sms;
+    return check_cuda(launch_pdl(kern, dim3((unsigned)grid), dim3(GEMV_THREADS), smem, stream, tm_w, p), "gemv_fp8 launch");
+}
+
+int gemv_fp8_codes(const uint8_t* a, const uint8_t* b, const Fp8GemmParams& g, cudaStream_t s) {
+    GemvParams p{};
+    p.g = g, p.a = a;
+    if (g.b_e5m2) return g.a_e5m2 ? launch_gemv<A_CODES, true, true>(b, p, s) : launch_gemv<A_CODES, true, false>(b, p, s);
+    return g.a_e5m2 ? launch_gemv<A_CODES, false, true>(b, p, s) : launch_gemv<A_CODES, false, false>(b, p, s);
+}
+int gemv_fp8_values(const void* x, bool f32, int64_t cols, const uint8_t* b, const Fp8GemmParams& g, cudaStream_t s) {
+    GemvParams p{};
+    p.g = g, p.a = static_cast<const uint8_t*>(x), p.a_cols = cols;
+    p.a_vec = aligned16(x) && cols % (f32 ? 4 : 8) == 0;
+    if (f32) return g.b_e5m2 ? launch_gemv<A_F32, true, false>(b, p, s) : launch_gemv<A_F32, false, false>(b, p, s);
+    return g.b_e5m2 ? launch_gemv<A_BF16, true, false>(b, p, s) : launch_gemv<A_BF16, false, false>(b, p, s);
+}
+
+QUARTET_DEFINE_STATUS_READER(status_gemv_fp8)
+
+}  // namespace quartet

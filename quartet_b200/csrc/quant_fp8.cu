@@ -13,7 +13,7 @@
 // One CTA takes 128 rows x 128 columns; eight threads share a row (16-byte loads, 128 bytes a row and load).  Bytes
 // per value: the input's 2 or 4, and 1 + 1/32 for each orientation written.
 #include "common.cuh"
-#include "quant_math.cuh"
+#include "quant_fp8.cuh"
 
 namespace quartet {
 
@@ -27,100 +27,6 @@ struct Fp8QuantParams {
     int top;                         // exponent of MAX: 8 (e4m3) or 15 (e5m2)
     int vec;                         // rows of x start on 16-byte boundaries
 };
-
-__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits, int top) {
-    if (amax_bits >= 0x7F800000u) return 255u;
-    const int b = (int)(amax_bits >> 23) - top + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return b < 0 ? 0u : (uint32_t)b;
-}
-// 2^(127 - b); b <= 247 here, so the exponent field stays positive
-__device__ __forceinline__ float fp8_inv_scale(uint32_t b) { return __uint_as_float((254u - b) << 23); }
-
-__device__ __forceinline__ uint32_t cvt_fp8x4(float a, float b, float c, float d, bool e5m2) {
-    uint16_t lo, hi;
-    if (e5m2) {
-        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    } else {
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    }
-    return (uint32_t)lo | ((uint32_t)hi << 16);
-}
-
-// Sixteen values of a row as 16-byte chunks j, j + 8 (bf16) or j, j + 8, j + 16, j + 24 (fp32) of the 128 columns; zeros
-// outside the tensor.
-template <bool F32>
-struct RowPart {
-    static constexpr int N = F32 ? 4 : 2, PER = F32 ? 4 : 8;
-    uint4 q[N];
-    __device__ __forceinline__ void load(const Fp8QuantParams& p, int64_t row, int64_t col0, int j) {
-        constexpr int EB = F32 ? 4 : 2;
-        const uint8_t* base = p.x + row * p.cols * EB;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t c = col0 + (j + 8 * i) * PER;
-            q[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (row >= p.rows) continue;
-            if (p.vec) {  // cols is a multiple of PER: a chunk is inside or outside as a whole
-                if (c < p.cols) q[i] = __ldg(reinterpret_cast<const uint4*>(base + c * EB));
-            } else {
-                uint32_t w[4] = {0u, 0u, 0u, 0u};
-                for (int k = 0; k < PER; ++k) {
-                    if (c + k >= p.cols) break;
-                    if (F32)
-                        w[k & 3] = __ldg(reinterpret_cast<const uint32_t*>(base) + c + k);
-                    else
-                        w[k >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(base) + c + k) << (16 * (k & 1));
-                }
-                q[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    }
-    __device__ __forceinline__ void chunk(int i, float (&v)[PER]) const {
-        if constexpr (F32) {
-            v[0] = __uint_as_float(q[i].x), v[1] = __uint_as_float(q[i].y), v[2] = __uint_as_float(q[i].z), v[3] = __uint_as_float(q[i].w);
-        } else {
-            unpack_bf16x8(q[i], v);
-        }
-    }
-    // bits of the largest magnitude: integer order is the order of magnitudes, infinities and NaN on top
-    __device__ __forceinline__ uint32_t amax() const {
-        uint32_t m = 0u;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float v[PER];
-            chunk(i, v);
-#pragma unroll
-            for (int k = 0; k < PER; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-        }
-        return m;
-    }
-    __device__ __forceinline__ void store_codes(uint8_t* row_codes, int j, uint32_t sb, bool e5m2) const {
-        const float inv = fp8_inv_scale(sb == 255u ? 127u : sb);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float v[PER];
-            chunk(i, v);
-            uint32_t w[PER / 4];
-#pragma unroll
-            for (int k = 0; k < PER / 4; ++k) {
-                w[k] = cvt_fp8x4(v[4 * k] * inv, v[4 * k + 1] * inv, v[4 * k + 2] * inv, v[4 * k + 3] * inv, e5m2);
-                if (sb == 255u) w[k] = 0x7F7F7F7Fu;
-            }
-            if constexpr (F32)
-                *reinterpret_cast<uint32_t*>(row_codes + (j + 8 * i) * PER) = w[0];
-            else
-                *reinterpret_cast<uint2*>(row_codes + (j + 8 * i) * PER) = make_uint2(w[0], w[1]);
-        }
-    }
-};
-
-__device__ __forceinline__ uint32_t max_over_8(uint32_t m) {
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    return m;
-}
 
 template <bool F32, bool SQUARE, bool ROWS, bool TRANS>
 constexpr int fp8_quant_smem() { return TRANS ? F8_TILE * F8_TILE * (F32 ? 4 : 2) + F8_TILE * F8_TILE + 8 * F8_TILE * 4 : 0; }
@@ -138,7 +44,7 @@ __global__ void __launch_bounds__(F8_THREADS) quant_fp8_kernel(const Fp8QuantPar
 
     RowPart<F32> part[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) part[s].load(p, row0 + r0 + 32 * s, col0, j);
+    for (int s = 0; s < 4; ++s) part[s].load(p.x, p.rows, p.cols, p.vec, row0 + r0 + 32 * s, col0, j);
 
     uint32_t tile_byte = 0;
     if constexpr (SQUARE) {
@@ -159,7 +65,11 @@ __global__ void __launch_bounds__(F8_THREADS) quant_fp8_kernel(const Fp8QuantPar
         for (int s = 0; s < 4; ++s) {
             const int r = r0 + 32 * s;
             const uint32_t sb = SQUARE ? tile_byte : fp8_scale_byte(max_over_8(part[s].amax()), p.top);
-            if (row0 + r < p.rows) part[s].store_codes(p.codes + (row0 + r) * p.pitch + col0, j, sb, e5m2);
+            if (row0 + r < p.rows) {
+                uint8_t* dst = p.codes + (row0 + r) * p.pitch + col0;
+#pragma unroll
+                for (int i = 0; i < RowPart<F32>::N; ++i) part[s].store_codes(dst + (j + 8 * i) * RowPart<F32>::PER, i, sb, e5m2);
+            }
             if (j == 0) *reinterpret_cast<uint32_t*>(sf + (r & 31) * 16 + (r >> 5) * 4) = row0 + r < p.rows ? sb * 0x01010101u : 0u;
         }
     }

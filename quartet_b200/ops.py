@@ -503,13 +503,28 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
     """x [..., K] times a packed weight (codes [N, pad128(K)] and scales of quant_fp8(weight, square=True)) -> [..., N]: x is quantized in
     blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear."""
     _need_codes(w, w_sf, "linear_fp8")
-    K = x.shape[-1]
-    if _pad128(K) != w.shape[1]:
+    shape, dev = x.shape, w.device
+    K, N = shape[-1], w.shape[0]
+    if (K + 127) // 128 * 128 != w.shape[1]:
         raise ValueError(f"x has {K} columns, the weight {w.shape[1]}")
-    x2 = x.reshape(-1, K)
-    xc, xs, _, _ = quant_fp8(x2 if x2.is_contiguous() else x2.contiguous())
-    y = gemm_fp8_tn(xc, xs, w, w_sf, out_dtype=out_dtype or x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+    if x.device != dev:
+        raise ValueError("x and the weight are on different devices")
+    if not x.is_contiguous():
+        x = x.contiguous()
+    M = x.numel() // K
+    dtype = out_dtype or x.dtype
+    xd, wd, yd = _dt(x), _f8(w.dtype), _out_dt(dtype)
+    y, pitch = _padded_out(M, N, dtype, dev)
+    if M and N:
+        lib = _lib.load()
+        nbytes = lib.quartet_linear_fp8_workspace_bytes(M, K)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _on(dev):
+            rc = lib.quartet_linear_fp8(x.data_ptr(), xd, M, K, w.data_ptr(), w_sf.data_ptr(), wd, N, 1.0, None if work is None else work.data_ptr(),
+                                        y.data_ptr(), yd, pitch, _stream())
+        if rc:
+            _lib.check(rc, "quartet_linear_fp8")
+    return y if len(shape) == 2 else y.view(*shape[:-1], N)
 
 
 # ------------------------------------------------------------------------------------------------

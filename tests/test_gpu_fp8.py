@@ -134,6 +134,31 @@ def test_product_of_mixed_formats(ops, fa, fb):
     _product(ops, 512, 768, 900, fa, fb)
 
 
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 40, 300])
+@pytest.mark.parametrize("K,N", [(1, 1), (127, 130), (640, 515), (1000, 64), (4096, 300), (2300, 1025)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_packed_weight_equals_quantizer_then_product(ops, M, K, N, dtype):
+    """The one-call form and, for few rows, the one-launch form: the same codes, so the same sums up to their order."""
+    x = _x(M, K, dtype, M + K)
+    if K > 300:
+        x[0, 299] = float("nan")
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(N)) * 0.02
+    wc, ws = ops.quant_fp8(w.cuda(), square=True)[:2]
+    y = ops.linear_fp8(x.cuda(), wc, ws)
+    y32 = ops.linear_fp8(x.cuda(), wc, ws, torch.float32)
+    assert y.dtype == dtype and y.shape == (M, N)
+    keep = x.clone()
+    if K > 300:
+        assert bool(torch.isnan(y[0]).all())
+        keep[0] = 0
+    xv, wv = fo.values(keep, E4M3), fo.values(w, E4M3, True)
+    want, s = xv @ wv.T, xv.abs() @ wv.abs().T
+    rows = slice(1, None) if K > 300 else slice(None)
+    for got, dt in ((y, dtype), (y32, torch.float32)):
+        assert bool(((got.cpu().double() - want).abs() <= _bound(s, fo.pad128(K), want, dt))[rows].all())
+    assert ops.device_status() == 0
+
+
 def test_product_takes_a_scale_for_every_32(ops):
     """The product itself reads one scale byte per 32 values: scales that differ inside a block of 128 count."""
     from oracle import ref_math as rm
@@ -253,7 +278,7 @@ def test_layer_shapes_strides_streams_and_empty_batches(ops):
     fp8_linear(xr, frozen).sum().backward()
     assert xr.grad is not None
     codes, sf = lin.export_fp8()
-    assert torch.equal(ops.linear_fp8(x, codes, sf), fp8_linear(x, frozen))
+    assert torch.allclose(ops.linear_fp8(x, codes, sf).float(), fp8_linear(x, frozen).float(), rtol=2.0 ** -7, atol=1e-5)
     assert ops.linear_fp8(x[:0], codes, sf).shape == (0, 3, 77)
     assert list(lin.state_dict()) == ["weight", "bias"]
 

@@ -60,6 +60,22 @@ def test_gemm_fp8_refusals(lib, p):
     assert f(ldd=7) == -2 and f(N=9, ldd=8) == -2 and f(N=9, ldd=12) == -2 and f(N=9, ldd=10, dt=1) == -2
 
 
+def test_linear_fp8_refusals(lib, p):
+    def f(x=p(), xd=0, M=4, K=200, w=p(), sf=p(), wd=0, N=8, work=p(), y=p(), yd=0, ldy=8):
+        return lib.quartet_linear_fp8(x, xd, M, K, w, sf, wd, N, 1.0, work, y, yd, ldy, None)
+
+    assert lib.quartet_linear_fp8_workspace_bytes(8, 200) == 0 and lib.quartet_linear_fp8_workspace_bytes(9, 200) == 9 * 256 + 128 * 8
+    for M in (4, 40):
+        for name in ("x", "w", "sf", "y"):
+            assert f(M=M, **{name: None}) == -1
+        for name in ("w", "sf", "y"):
+            assert f(M=M, **{name: p(8)}) == -3
+        assert f(M=M, x=p(1)) == -3 and f(M=M, x=p(2), xd=1) == -3
+        assert f(M=M, xd=2) == -4 and f(M=M, wd=2) == -4 and f(M=M, yd=2) == -4
+        assert f(M=M, N=0) == -2 and f(M=M, K=0) == -2 and f(M=M, N=9) == -2 and f(M=M, ldy=12) == -2
+    assert f(M=0) == -2 and f(M=8388481) == -2 and f(M=9, work=None) == -1 and f(M=9, work=p(8)) == -3
+
+
 def test_rotary_refusals(lib, p):
     def f(n=1, src=(p(),), dst=(p(1024),), strides=(0,) * 18, heads=(1,), rotate=(1,), dt=0, batch=1, tokens=1, d=64, rot=64, pos=None, i64=1, inv=p(2048)):
         m = max(len(src), 1)
