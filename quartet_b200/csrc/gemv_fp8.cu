@@ -133,13 +133,13 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t sb = fp8_scale_byte(max_over_8(part[u].amax()), 8);
+                const uint32_t sb = fp8_scale_byte(mag_over_8<AMODE == A_F32>(part[u].mag()), 8);
                 if (at[u] >= n) continue;
                 const int r = at[u] / chunks, c = at[u] - r * chunks;
 #pragma unroll
                 for (int q = 0; q < R::N; ++q) {
                     uint32_t w[R::PER / 4];
-                    part[u].codes(w, q, sb, false);
+                    part[u].template codes<false>(w, q, fp8_inv_scale(sb));
                     uint2* dst = reinterpret_cast<uint2*>(s_a + r * pitch + c * 256 + (j + 8 * q) * R::PER * 2);
 #pragma unroll
                     for (int k = 0; k < R::PER / 4; ++k) dst[k] = make_uint2(f16x2_of<false>(w[k]), f16x2_of<false>(w[k] >> 16));
