@@ -7,15 +7,17 @@
 // the split of a packed projection into heads -- and, backward, its join -- is the same pass over memory as the rotation.
 //
 // Angles: the turn pos * inv_freq / 2 pi is taken in 64 bits and reduced there, because in 32 bits a position of 2^17 leaves an angle
-// 2^-7 wrong; its fraction goes to sincospif, with the part that 32 bits lose put back to first order.  A CTA computes the
-// rot / 2 pairs of its token once, in shared memory, and every head uses them: the angles cost no memory traffic.
+// 2^-7 wrong; its fraction goes to sincospif, with the part that 32 bits lose put back to first order.  They cost no memory traffic
+// and no table in it: a thread owns the same few pairs of a token in all heads, computes their sines and cosines once, keeps them in
+// registers and walks the heads, four at a time.  Where there are few tokens a thread takes every split-th head, and the threads of a token
+// share its pairs through shared memory.
 // Bound by memory: each value is read and written once.
 #include "common.cuh"
 #include "quant_math.cuh"
 
 namespace quartet {
 
-constexpr int ROT_THREADS = 128, ROT_MAX_PAIRS = 256, ROT_MAX_SEGS = 3;
+constexpr int ROT_THREADS = 256, ROT_MAX_PAIRS = 256, ROT_MAX_SEGS = 3;
 
 struct RotSeg {
     const void* src;
@@ -33,26 +35,41 @@ struct RotParams {
     const double* inv_freq;
     float scale;
     int inverse;
+    int64_t tokens;
+    int lanes, split, per_block;  // threads a token and head group, head groups, tokens of a block
 };
 
 // Values one thread moves at a time: 16 bytes where every row allows it, single values otherwise.
 template <bool F32, bool VEC>
 struct RotVec {
     static constexpr int N = VEC ? (F32 ? 4 : 8) : 1;
-    float v[N];
+    uint4 q;
     __device__ __forceinline__ void load(const void* p, int64_t i) {
-        if constexpr (VEC && F32) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
-            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-        } else if constexpr (VEC) {
-            unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i)), v);
-        } else if constexpr (F32) {
-            v[0] = __ldg(static_cast<const float*>(p) + i);
+        if constexpr (VEC)
+            q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (F32 ? 4 : 2)));
+        else if constexpr (F32)
+            q.x = __ldg(static_cast<const uint32_t*>(p) + i);
+        else
+            q.x = (uint32_t)__ldg(static_cast<const uint16_t*>(p) + i) << 16;
+    }
+    __device__ __forceinline__ void copy(void* p, int64_t i) const {
+        if constexpr (VEC)
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * (F32 ? 4 : 2)) = q;
+        else if constexpr (F32)
+            static_cast<uint32_t*>(p)[i] = q.x;
+        else
+            static_cast<uint16_t*>(p)[i] = (uint16_t)(q.x >> 16);
+    }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+        if constexpr (VEC && !F32) {
+            unpack_bf16x8(q, v);
         } else {
-            v[0] = __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(p) + i) << 16);
+            const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = __uint_as_float(r[k]);
         }
     }
-    __device__ __forceinline__ void store(void* p, int64_t i) const {
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[N]) {
         if constexpr (VEC && F32) {
             *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
         } else if constexpr (VEC) {
@@ -71,70 +88,117 @@ struct RotVec {
     }
 };
 
-template <bool F32, bool INTERLEAVED, bool VEC>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotParams p) {
-    __shared__ __align__(16) float s_cos[ROT_MAX_PAIRS], s_sin[ROT_MAX_PAIRS];
+__device__ __forceinline__ int64_t position(const RotParams& p, int64_t token) {
+    const int64_t b = (uint32_t)token / (uint32_t)p.T, t = token - b * p.T;
+    if (!p.pos) return p.offset + t;
+    const int64_t at = b * p.pos_b + t * p.pos_t;
+    return p.pos_i64 ? (int64_t)__ldg(static_cast<const long long*>(p.pos) + at) : (int64_t)__ldg(static_cast<const int*>(p.pos) + at);
+}
+// (cosine, sine) of a pair at a position, times the scale
+__device__ __forceinline__ float2 rotation(const RotParams& p, int64_t pos, int pair) {
+    double turn = (double)pos * (__ldg(p.inv_freq + pair) * 0.15915494309189533577);
+    turn = 2.0 * (turn - rint(turn));  // half turns, in [-1, 1]
+    const float hi = (float)turn, lo = (float)(turn - (double)hi) * 3.14159265f;
+    float s, c;
+    sincospif(hi, &s, &c);
+    return make_float2((c - s * lo) * p.scale, (s + c * lo) * (p.inverse ? -p.scale : p.scale));
+}
+
+template <bool F32, bool INTERLEAVED, bool VEC, bool SPLIT>
+__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotParams p) {
     using V = RotVec<F32, VEC>;
+    // a unit is what a thread moves at once: one vector of side-by-side pairs, two vectors half a rotated part apart (two single
+    // values, in either layout), or one vector that is only copied
+    constexpr bool ONE = INTERLEAVED && VEC;
+    constexpr int RU = ONE ? V::N : 2 * V::N, PAIRS = RU / 2;
+    const int ru = p.rot / RU, units = ru + (p.d - p.rot) / V::N;
+    // Heads in flight.  Many tokens: four (two, for the layout with two vectors a unit: 75 us against 56 at 32768 tokens of 15 heads).  Few
+    // tokens leave a thread few heads, and registers are worth more as resident threads: 3063 tokens of 12 fp32 heads 10.3 us with four, 7.3 with two.
+    constexpr int ROT_AHEAD = SPLIT ? 2 : 4;
+    extern __shared__ __align__(16) float2 s_cs[];  // [token of the block][pair]
+    const int lane = threadIdx.x % p.lanes, rest = threadIdx.x / p.lanes, group = rest % p.split, mine = rest / p.split;
     const int pairs = p.rot >> 1;
-    const int64_t token = blockIdx.x, b = token / p.T, t = token - b * p.T;
+    const int64_t token = (int64_t)blockIdx.x * p.per_block + mine;
     pdl_launch_dependents();
     pdl_wait();
-    int64_t pos = p.offset + t;
-    if (p.pos) {
-        const int64_t at = b * p.pos_b + t * p.pos_t;
-        pos = p.pos_i64 ? (int64_t)__ldg(static_cast<const long long*>(p.pos) + at) : (int64_t)__ldg(static_cast<const int*>(p.pos) + at);
+    if constexpr (SPLIT) {
+        for (int i = threadIdx.x; i < p.per_block * pairs; i += blockDim.x) {
+            const int64_t tok = (int64_t)blockIdx.x * p.per_block + i / pairs;
+            if (tok >= p.tokens) break;
+            s_cs[i] = rotation(p, position(p, tok), i % pairs);
+        }
+        __syncthreads();
     }
-    for (int i = threadIdx.x; i < pairs; i += ROT_THREADS) {
-        double turn = (double)pos * (p.inv_freq[i] * 0.15915494309189533577);
-        turn = 2.0 * (turn - rint(turn));  // half turns, in [-1, 1]
-        const float hi = (float)turn, lo = (float)(turn - (double)hi) * 3.14159265f;
-        float s, c;
-        sincospif(hi, &s, &c);
-        const float c2 = c - s * lo, s2 = s + c * lo;
-        s_cos[i] = c2 * p.scale;
-        s_sin[i] = (p.inverse ? -s2 : s2) * p.scale;
-    }
-    __syncthreads();
-    // a unit is what a thread moves at once: one vector of side-by-side pairs, two vectors half a rotated part apart, or
-    // one vector that is only copied
-    constexpr int RU = INTERLEAVED ? (VEC ? V::N : 2) : 2 * V::N;  // values of a rotated unit
+    if (token >= p.tokens) return;
+    const int64_t pos = SPLIT ? 0 : position(p, token);
+    const int64_t b = (uint32_t)token / (uint32_t)p.T, t = token - b * p.T;
+    for (int i = lane; i < units; i += p.lanes) {
+        const bool turns = i < ru;
+        const int a1 = !turns ? p.rot + (i - ru) * V::N : ONE ? i * RU : (INTERLEAVED ? 2 * i : i * V::N);
+        const int a2 = INTERLEAVED ? a1 + 1 : a1 + (p.rot >> 1);  // (second vector of a unit that has two)
+        float cs[PAIRS], sn[PAIRS];
+        if (turns) {
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+                const float2 v = SPLIT ? s_cs[mine * pairs + i * PAIRS + k] : rotation(p, pos, i * PAIRS + k);
+                cs[k] = v.x, sn[k] = v.y;
+            }
+        }
 #pragma unroll 1
-    for (int g = 0; g < p.n_seg; ++g) {
-        const RotSeg& sg = p.seg[g];
-        const int turned = sg.rotate ? p.rot : 0;
-        const int ru = turned / RU, units = ru + (p.d - turned) / V::N, total = units * sg.heads;
-        const int64_t so = b * sg.s_b + t * sg.s_t, to = b * sg.d_b + t * sg.d_t;
-        for (int u = threadIdx.x; u < total; u += ROT_THREADS) {
-            const int h = u / units, i = u - h * units;
-            const int64_t sh = so + h * sg.s_h, dh = to + h * sg.d_h;
-            if (i >= ru) {
-                V x;
-                const int at = turned + (i - ru) * V::N;
-                x.load(sg.src, sh + at);
-                x.store(sg.dst, dh + at);
-            } else if constexpr (INTERLEAVED && VEC) {
-                V x, y;
-                x.load(sg.src, sh + i * RU);
+        for (int g = 0; g < p.n_seg; ++g) {
+            const RotSeg& sg = p.seg[g];
+            const int64_t so = b * sg.s_b + t * sg.s_t, to = b * sg.d_b + t * sg.d_t;
+            if (!sg.rotate || !turns) {
+                // copied: the vector past the rotated part, or (v) this thread's share of whole heads
+                const int first = sg.rotate ? a1 : i * V::N, last = sg.rotate ? a1 + 1 : p.d, step = units * V::N;
+                for (int at = first; at < last; at += step) {
+#pragma unroll 1
+                    for (int h0 = group; h0 < sg.heads; h0 += ROT_AHEAD * p.split) {
+                        V x[ROT_AHEAD];
 #pragma unroll
-                for (int k = 0; k < V::N / 2; ++k) {
-                    const float c = s_cos[i * (RU / 2) + k], s = s_sin[i * (RU / 2) + k];
-                    y.v[2 * k] = x.v[2 * k] * c - x.v[2 * k + 1] * s;
-                    y.v[2 * k + 1] = x.v[2 * k] * s + x.v[2 * k + 1] * c;
-                }
-                y.store(sg.dst, dh + i * RU);
-            } else {
-                const int a1 = INTERLEAVED ? 2 * i : i * V::N, a2 = INTERLEAVED ? 2 * i + 1 : pairs + i * V::N;
-                V x1, x2, y1, y2;
-                x1.load(sg.src, sh + a1);
-                x2.load(sg.src, sh + a2);
+                        for (int u = 0; u < ROT_AHEAD; ++u)
+                            if (h0 + u * p.split < sg.heads) x[u].load(sg.src, so + (h0 + u * p.split) * sg.s_h + at);
 #pragma unroll
-                for (int k = 0; k < V::N; ++k) {
-                    const float c = s_cos[i * V::N + k], s = s_sin[i * V::N + k];
-                    y1.v[k] = x1.v[k] * c - x2.v[k] * s;
-                    y2.v[k] = x1.v[k] * s + x2.v[k] * c;
+                        for (int u = 0; u < ROT_AHEAD; ++u)
+                            if (h0 + u * p.split < sg.heads) x[u].copy(sg.dst, to + (h0 + u * p.split) * sg.d_h + at);
+                    }
                 }
-                y1.store(sg.dst, dh + a1);
-                y2.store(sg.dst, dh + a2);
+                continue;
+            }
+#pragma unroll 1
+            for (int h0 = group; h0 < sg.heads; h0 += ROT_AHEAD * p.split) {
+                V x1[ROT_AHEAD], x2[ROT_AHEAD];
+#pragma unroll
+                for (int u = 0; u < ROT_AHEAD; ++u)
+                    if (h0 + u * p.split < sg.heads) {
+                        const int64_t at = so + (h0 + u * p.split) * sg.s_h;
+                        x1[u].load(sg.src, at + a1);
+                        if (!ONE) x2[u].load(sg.src, at + a2);
+                    }
+#pragma unroll
+                for (int u = 0; u < ROT_AHEAD; ++u)
+                    if (h0 + u * p.split < sg.heads) {
+                        const int64_t at = to + (h0 + u * p.split) * sg.d_h;
+                        float v1[V::N], y1[V::N];
+                        x1[u].get(v1);
+                        if constexpr (ONE) {
+#pragma unroll
+                            for (int k = 0; k < PAIRS; ++k) {
+                                y1[2 * k] = v1[2 * k] * cs[k] - v1[2 * k + 1] * sn[k];
+                                y1[2 * k + 1] = v1[2 * k] * sn[k] + v1[2 * k + 1] * cs[k];
+                            }
+                        } else {
+                            float v2[V::N], y2[V::N];
+                            x2[u].get(v2);
+#pragma unroll
+                            for (int k = 0; k < PAIRS; ++k) {
+                                y1[k] = v1[k] * cs[k] - v2[k] * sn[k];
+                                y2[k] = v1[k] * sn[k] + v2[k] * cs[k];
+                            }
+                            V::store(sg.dst, at + a2, y2);
+                        }
+                        V::store(sg.dst, at + a1, y1);
+                    }
             }
         }
     }
@@ -144,10 +208,24 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotParams p) 
 // host
 // ---------------------------------------------------------------------------
 template <bool F32>
-static int launch_rotary(const RotParams& p, int64_t tokens, bool interleaved, bool vec, cudaStream_t s) {
-    void (*kern)(const RotParams) = interleaved ? (vec ? rotary_kernel<F32, true, true> : rotary_kernel<F32, true, false>)
-                                                : (vec ? rotary_kernel<F32, false, true> : rotary_kernel<F32, false, false>);
-    return check_cuda(launch_pdl(kern, dim3((unsigned)tokens), dim3(ROT_THREADS), 0, s, p), "rotary launch");
+static int launch_rotary(RotParams p, bool interleaved, bool vec, cudaStream_t s) {
+    int rc, sms = 0, heads = 1;
+    if ((rc = device_sm_count(&sms))) return rc;
+    const int n = vec ? (F32 ? 4 : 8) : 1, ru = interleaved && vec ? n : 2 * n;
+    const int units = p.rot / ru + (p.d - p.rot) / n;
+    p.lanes = units < ROT_THREADS ? units : ROT_THREADS;
+    for (int g = 0; g < p.n_seg; ++g) heads = p.seg[g].heads > heads ? p.seg[g].heads : heads;
+    // Head groups: one, so that a pair's sine and cosine are computed once, unless the threads would then be fewer than fill the GPU (a new
+    // token of each sequence).
+    p.split = 1;
+    while (p.split < heads && 2 * p.split * p.lanes <= ROT_THREADS && p.tokens * p.split * p.lanes < (int64_t)sms * 1024) p.split *= 2;
+    p.per_block = ROT_THREADS / (p.lanes * p.split);
+    const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
+    void (*const kerns[2][2][2])(const RotParams) = {
+        {{rotary_kernel<F32, false, false, false>, rotary_kernel<F32, false, false, true>}, {rotary_kernel<F32, false, true, false>, rotary_kernel<F32, false, true, true>}},
+        {{rotary_kernel<F32, true, false, false>, rotary_kernel<F32, true, false, true>}, {rotary_kernel<F32, true, true, false>, rotary_kernel<F32, true, true, true>}}};
+    const auto kern = kerns[interleaved][vec][p.split > 1];
+    return check_cuda(launch_pdl(kern, dim3((unsigned)blocks), dim3(p.lanes * p.split * p.per_block), p.split > 1 ? (size_t)p.per_block * (p.rot / 2) * sizeof(float2) : 0, s, p), "rotary launch");
 }
 
 }  // namespace quartet
@@ -189,5 +267,6 @@ extern "C" __attribute__((visibility("default"))) int quartet_rotary(int n_seg, 
     p.pos = pos, p.pos_i64 = pos_i64, p.pos_b = pos_stride_b, p.pos_t = pos_stride_t, p.offset = offset;
     p.inv_freq = inv_freq, p.scale = scale, p.inverse = inverse != 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return f32 ? launch_rotary<true>(p, batch * tokens, interleaved != 0, vec, s) : launch_rotary<false>(p, batch * tokens, interleaved != 0, vec, s);
+    p.tokens = batch * tokens;
+    return f32 ? launch_rotary<true>(p, interleaved != 0, vec, s) : launch_rotary<false>(p, interleaved != 0, vec, s);
 }
