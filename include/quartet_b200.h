@@ -270,6 +270,19 @@ int quartet_linear_fp8(const void* x, int x_dtype, int64_t M, int64_t K, const u
                        uint8_t* workspace, void* y, int y_dtype, int64_t ldy, quartet_stream_t stream);
 
 /*
+ * The whole 8-bit layer in one host call per direction (the kernels above in order; x, w, e contiguous).
+ * quartet_linear_fp8_train_bytes: bytes3 (host) = {saved, forward workspace, backward workspace} for the gradients that are wanted.
+ * ..._fwd: y [M, N] = Q(x [M, K]) Q(w [N, K])^T; saved receives the transposes that dx (w's) and dw (x's) need.
+ * ..._bwd: dx [M, K] and / or dw [N, K] (NULL: not computed; workspace for those alone suffices) from e [M, N] quantized to fmt; saved_dx, saved_dw:
+ * the forward's need_dx, need_dw.  M, N, K in 1 .. 8388480; buffers 16-byte aligned; pitches as in quartet_gemm_fp8_tn.
+ */
+int quartet_linear_fp8_train_bytes(int64_t M, int64_t N, int64_t K, int need_dx, int need_dw, int64_t* bytes3);
+int quartet_linear_fp8_train_fwd(const void* x, int x_dtype, const void* w, int w_dtype, int64_t M, int64_t N, int64_t K, int need_dx, int need_dw,
+                                 uint8_t* saved, uint8_t* workspace, void* y, int y_dtype, int64_t ldy, quartet_stream_t stream);
+int quartet_linear_fp8_train_bwd(const void* e, int e_dtype, int64_t M, int64_t N, int64_t K, int fmt, const uint8_t* saved, uint8_t* workspace, void* dx,
+                                 int dx_dtype, int64_t ldx, void* dw, int dw_dtype, int64_t ldw, int saved_dx, int saved_dw, quartet_stream_t stream);
+
+/*
  * Rotary positions (applied to q and k in LlamaAttention, src/models/llama.py:117-158): in every head, pair i of the first `rot` of d values turns
  * by pos * inv_freq[i], the result times `scale`; the other values are copied.  interleaved 1: pairs (2 i, 2 i + 1), the reference's
  * layout; 0: pairs (i, i + rot / 2).  inverse 1: by the negative angle (the gradient).

@@ -49,6 +49,9 @@ SIGNATURES = {
     "quartet_gemm_fp8_tn": (_i, [_p, _p, _i, _p, _p, _i, _i64, _i64, _i64, _f, _p, _i, _i64, _p]),
     "quartet_linear_fp8_workspace_bytes": (_i64, [_i64, _i64]),
     "quartet_linear_fp8": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i64, _f, _p, _p, _i, _i64, _p]),
+    "quartet_linear_fp8_train_bytes": (_i, [_i64, _i64, _i64, _i, _i, _p]),
+    "quartet_linear_fp8_train_fwd": (_i, [_p, _i, _p, _i, _i64, _i64, _i64, _i, _i, _p, _p, _p, _i, _i64, _p]),
+    "quartet_linear_fp8_train_bwd": (_i, [_p, _i, _i64, _i64, _i64, _i, _p, _p, _p, _i, _i64, _p, _i, _i64, _i, _i, _p]),
     "quartet_rotary": (_i, [_i, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _i64, _i, _p, _i, _i64, _i64, _i64, _p, _f, _i, _p]),
     "quartet_grad_norm": (_i, [C.c_int32, _p, _p, _p, _i, _p, _p, _p, _p]),
     "quartet_clip_grads": (_i, [C.c_int32, _p, _p, _p, _p, _p, _i, C.c_double, _p, _p, _p, _p]),

@@ -3,6 +3,7 @@ current stream; all arithmetic happens in libquartet_b200.so."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from array import array
 
@@ -525,6 +526,51 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
         if rc:
             _lib.check(rc, "quartet_linear_fp8")
     return y if len(shape) == 2 else y.view(*shape[:-1], N)
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp8_train_bytes(M, N, K, need_dx, need_dw):
+    out = (C.c_int64 * 3)()
+    _lib.check(_lib.load().quartet_linear_fp8_train_bytes(M, N, K, need_dx, need_dw, C.addressof(out)), "quartet_linear_fp8_train_bytes")
+    return tuple(out)
+
+
+def fp8_linear_fwd(x2, w, need_dx, need_dw, out_dtype):
+    """x2 [M, K], w [N, K] -> (y [M, N], saved): the 8-bit layer's forward in one call; saved is what fp8_linear_bwd takes."""
+    _need_cuda(x2, w)
+    (M, K), N, dev = x2.shape, w.shape[0], x2.device
+    xd, wd, yd = _dt(x2), _dt(w), _out_dt(out_dtype)
+    y, pitch = _padded_out(M, N, out_dtype, dev)
+    need_dx, need_dw = 1 if need_dx else 0, 1 if need_dw else 0
+    if not (M and N and K):
+        return y.zero_(), torch.empty(0, dtype=torch.uint8, device=dev)
+    saved_bytes, work_bytes, _ = _fp8_train_bytes(M, N, K, need_dx, need_dw)
+    saved, work = torch.empty(saved_bytes, dtype=torch.uint8, device=dev), torch.empty(work_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = _lib.load().quartet_linear_fp8_train_fwd(x2.data_ptr(), xd, w.data_ptr(), wd, M, N, K, need_dx, need_dw, saved.data_ptr() if saved_bytes else None,
+                                                      work.data_ptr(), y.data_ptr(), yd, pitch, _stream())
+    if rc:
+        _lib.check(rc, "quartet_linear_fp8_train_fwd")
+    return y, saved
+
+
+def fp8_linear_bwd(e2, saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw, saved_dx, saved_dw):
+    """e2 [M, N] and the forward's saved buffer (made with need_dx = saved_dx, need_dw = saved_dw) -> (dx [M, K] | None, dw [N, K] | None)."""
+    _need_cuda(e2, saved)
+    (M, N), dev = e2.shape, e2.device
+    ed, fmt = _dt(e2), _f8(grad_dtype)
+    dx, ldx = _padded_out(M, K, x_dtype, dev) if need_dx else (None, 0)
+    dw, ldw = _padded_out(N, K, w_dtype, dev) if need_dw else (None, 0)
+    if not (M and N and K):
+        return None if dx is None else dx.zero_(), None if dw is None else dw.zero_()
+    work = torch.empty(_fp8_train_bytes(M, N, K, 1 if need_dx else 0, 1 if need_dw else 0)[2], dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = _lib.load().quartet_linear_fp8_train_bwd(e2.data_ptr(), ed, M, N, K, fmt, saved.data_ptr(), work.data_ptr(), dx.data_ptr() if need_dx else None,
+                                                      _out_dt(x_dtype), ldx, dw.data_ptr() if need_dw else None, _out_dt(w_dtype), ldw, 1 if saved_dx else 0,
+                                                      1 if saved_dw else 0, _stream())
+    if rc:
+        _lib.check(rc, "quartet_linear_fp8_train_bwd")
+    return dx, dw
 
 
 # ------------------------------------------------------------------------------------------------

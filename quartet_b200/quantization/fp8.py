@@ -20,35 +20,29 @@ from .producers import _out_dtype
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, grad_dtype, out_dtype):
-        K, (need_dx, need_dw) = w.shape[1], ctx.needs_input_grad[:2]
-        x2 = x.reshape(-1, K)
-        xc, xs, xtc, xts = ops.quant_fp8(x2 if x2.is_contiguous() else x2.contiguous(), transpose=need_dw)
-        wc, ws, wtc, wts = ops.quant_fp8(w if w.is_contiguous() else w.contiguous(), square=True, transpose=need_dx)
-        y = ops.gemm_fp8_tn(xc, xs, wc, ws, out_dtype=out_dtype)
-        ctx.save_for_backward(xtc, xts, wtc, wts)
-        ctx.x_shape, ctx.dtypes = x.shape, (grad_dtype, x.dtype, w.dtype)
-        return y.view(*x.shape[:-1], w.shape[0])
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        x2 = x if x.dim() == 2 else x.reshape(-1, w.shape[1])
+        y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
+        ctx.save_for_backward(saved)
+        ctx.x_shape, ctx.args, ctx.kept = x.shape, (w.shape[1], grad_dtype, x.dtype, w.dtype), (need_dx, need_dw)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     def backward(ctx, e):
         if torch.is_grad_enabled():
             raise RuntimeError("fp8_linear is not differentiable twice")
-        xtc, xts, wtc, wts = ctx.saved_tensors
-        grad_dtype, x_dtype, w_dtype = ctx.dtypes
         need_dx, need_dw = ctx.needs_input_grad[:2]
         if not (need_dx or need_dw):
             return None, None, None, None
-        e2 = e.reshape(-1, e.shape[-1])
+        e2 = e if e.dim() == 2 else e.reshape(-1, e.shape[-1])
         if e2.dtype not in (torch.bfloat16, torch.float32):
             e2 = e2.float()
-        ec, es, etc, ets = ops.quant_fp8(e2 if e2.is_contiguous() else e2.contiguous(), grad_dtype, rows=need_dx, transpose=need_dw)
-        dx = dw = None
-        if need_dx:
-            dx = ops.gemm_fp8_tn(ec, es, wtc, wts, out_dtype=x_dtype).view(ctx.x_shape)
-        if need_dw:
-            dw = ops.gemm_fp8_tn(etc, ets, xtc, xts, out_dtype=w_dtype).contiguous()
-        ops.raise_on_fault("8-bit linear backward")  # only with QUARTET_CHECK_FAULTS=1
-        return dx, dw, None, None
+        dx, dw = ops.fp8_linear_bwd(e2 if e2.is_contiguous() else e2.contiguous(), ctx.saved_tensors[0], *ctx.args, need_dx, need_dw, *ctx.kept)
+        if ops.CHECK_FAULTS:
+            ops.raise_on_fault("8-bit linear backward")
+        if dx is not None and len(ctx.x_shape) != 2:
+            dx = dx.view(ctx.x_shape)
+        return dx, (dw if dw is None or dw.is_contiguous() else dw.contiguous()), None, None
 
 
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, grad_dtype: torch.dtype = torch.float8_e4m3fn, out_dtype: torch.dtype | None = None) -> torch.Tensor:

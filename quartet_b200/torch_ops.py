@@ -536,64 +536,57 @@ torch.library.register_autograd("quartet_b200::rotary_qkv", _rotary_qkv_backward
 # the 8-bit block-scaled linear layer
 # ------------------------------------------------------------------------------------------------
 @torch.library.custom_op("quartet_b200::fp8_linear_fwd", mutates_args=())
-def fp8_linear_fwd(x: Tensor, w: Tensor, grad_dtype: torch.dtype, out_dtype: torch.dtype, need_dx: bool,
-                   need_dw: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """y = Q(x) Q(w)^T and what its backward needs: the codes and scales of x and w transposed (empty where not needed)."""
-    K = w.shape[1]
-    x2 = x.reshape(-1, K)
-    xc, xs, xtc, xts = ops.quant_fp8(x2 if x2.is_contiguous() else x2.contiguous(), transpose=need_dw)
-    wc, ws, wtc, wts = ops.quant_fp8(w if w.is_contiguous() else w.contiguous(), square=True, transpose=need_dx)
-    y = ops.gemm_fp8_tn(xc, xs, wc, ws, out_dtype=out_dtype).reshape(*x.shape[:-1], w.shape[0])
-    e8, e1 = xc.new_empty((0, 0)), xs.new_empty((0,))
-    return y.contiguous(), (e8 if xtc is None else xtc), (e1 if xts is None else xts), (e8.clone() if wtc is None else wtc), (e1.clone() if wts is None else wts)
+def fp8_linear_fwd(x: Tensor, w: Tensor, grad_dtype: torch.dtype, out_dtype: torch.dtype, need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
+    """y = Q(x) Q(w)^T and what its backward needs: codes and scales of x and w transposed, as one buffer."""
+    x2 = x.reshape(-1, w.shape[1])
+    y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
+    return y.reshape(*x.shape[:-1], w.shape[0]).contiguous(), saved
+
+
+def _pad256(n: int) -> int:
+    return (n + 255) // 256 * 256
 
 
 @fp8_linear_fwd.register_fake
 def _(x, w, grad_dtype, out_dtype, need_dx, need_dw):
     N, K = w.shape
-    m, f8 = x.numel() // K, torch.float8_e4m3fn
+    m = x.numel() // K
     mp, np_ = _pad128(m), _pad128(N)
-    return (x.new_empty((*x.shape[:-1], N), dtype=out_dtype),
-            x.new_empty((K, mp) if need_dw else (0, 0), dtype=f8), _u8(x, _sf_bytes(K, mp) if need_dw else 0),
-            x.new_empty((K, np_) if need_dx else (0, 0), dtype=f8), _u8(x, _sf_bytes(K, np_) if need_dx else 0))
+    saved = (_pad256(K * mp) + _pad256(_sf_bytes(K, mp)) if need_dw else 0) + (_pad256(K * np_) + _pad256(_sf_bytes(K, np_)) if need_dx else 0)
+    return x.new_empty((*x.shape[:-1], N), dtype=out_dtype), _u8(x, saved)
 
 
 @torch.library.custom_op("quartet_b200::fp8_linear_bwd", mutates_args=())
-def fp8_linear_bwd(e: Tensor, xtc: Tensor, xts: Tensor, wtc: Tensor, wts: Tensor, grad_dtype: torch.dtype, x_dtype: torch.dtype, w_dtype: torch.dtype,
-                   need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
+def fp8_linear_bwd(e: Tensor, saved: Tensor, K: int, grad_dtype: torch.dtype, x_dtype: torch.dtype, w_dtype: torch.dtype, need_dx: bool,
+                   need_dw: bool) -> Tuple[Tensor, Tensor]:
     """dx [m, K] = Q(e) Q(w) and dw [N, K] = Qt(e)^T Qt(x); empty where not needed."""
-    N = e.shape[-1]
-    e2 = e.reshape(-1, N)
+    e2 = e.reshape(-1, e.shape[-1])
     if e2.dtype not in (torch.bfloat16, torch.float32):
         e2 = e2.float()
-    ec, es, etc, ets = ops.quant_fp8(e2 if e2.is_contiguous() else e2.contiguous(), grad_dtype, rows=need_dx, transpose=need_dw)
-    dx = ops.gemm_fp8_tn(ec, es, wtc, wts, out_dtype=x_dtype).contiguous() if need_dx else e.new_empty((0,), dtype=x_dtype)
-    dw = ops.gemm_fp8_tn(etc, ets, xtc, xts, out_dtype=w_dtype).contiguous() if need_dw else e.new_empty((0,), dtype=w_dtype)
+    dx, dw = ops.fp8_linear_bwd(e2 if e2.is_contiguous() else e2.contiguous(), saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw, need_dx, need_dw)
     ops.raise_on_fault("8-bit linear backward")  # only with QUARTET_CHECK_FAULTS=1
-    return dx, dw
+    return (dx.contiguous() if need_dx else e.new_empty((0,), dtype=x_dtype)), (dw.contiguous() if need_dw else e.new_empty((0,), dtype=w_dtype))
 
 
 @fp8_linear_bwd.register_fake
-def _(e, xtc, xts, wtc, wts, grad_dtype, x_dtype, w_dtype, need_dx, need_dw):
+def _(e, saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw):
     N = e.shape[-1]
     m = e.numel() // N
-    dx = e.new_empty((m, wtc.shape[0]) if need_dx else (0,), dtype=x_dtype)
-    dw = e.new_empty((N, xtc.shape[0]) if need_dw else (0,), dtype=w_dtype)
-    return dx, dw
+    return e.new_empty((m, K) if need_dx else (0,), dtype=x_dtype), e.new_empty((N, K) if need_dw else (0,), dtype=w_dtype)
 
 
 def _fp8_linear_setup(ctx, inputs, output):
     x, w, grad_dtype, _, need_dx, need_dw = inputs
-    ctx.save_for_backward(*output[1:])
-    ctx.x_shape, ctx.args = x.shape, (grad_dtype, x.dtype, w.dtype, need_dx, need_dw)
+    ctx.save_for_backward(output[1])
+    ctx.x_shape, ctx.args = x.shape, (w.shape[1], grad_dtype, x.dtype, w.dtype, need_dx, need_dw)
     ctx.set_materialize_grads(False)
 
 
 def _fp8_linear_backward(ctx, e, *unused):
     if e is None:
         return (None,) * 6
-    dx, dw = torch.ops.quartet_b200.fp8_linear_bwd(e, *ctx.saved_tensors, *ctx.args)
-    need_dx, need_dw = ctx.args[3:]
+    dx, dw = torch.ops.quartet_b200.fp8_linear_bwd(e, ctx.saved_tensors[0], *ctx.args)
+    need_dx, need_dw = ctx.args[4:]
     return (dx.reshape(ctx.x_shape) if need_dx else None), (dw if need_dw else None), None, None, None, None
 
 

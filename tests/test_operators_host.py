@@ -76,6 +76,36 @@ def test_linear_fp8_refusals(lib, p):
     assert f(M=0) == -2 and f(M=8388481) == -2 and f(M=9, work=None) == -1 and f(M=9, work=p(8)) == -3
 
 
+def test_layer_refusals(lib, p):
+    b3 = (C.c_int64 * 3)()
+    assert lib.quartet_linear_fp8_train_bytes(0, 1, 1, 1, 1, b3) == -2 and lib.quartet_linear_fp8_train_bytes(1, 1, 1, 1, 1, None) == -1
+    assert lib.quartet_linear_fp8_train_bytes(200, 100, 300, 1, 1, b3) == 0
+    xt, wt = 300 * 256 + 384 * 8, 300 * 128 + 384 * 4          # transposes of x and w: codes and scales, in 256-byte units
+    assert list(b3) == [xt + wt, 200 * 384 + 256 * 12 + 100 * 384 + 128 * 12, 200 * 128 + 256 * 4 + 100 * 256 + 128 * 8]
+    assert lib.quartet_linear_fp8_train_bytes(200, 100, 300, 0, 0, b3) == 0 and b3[0] == 0 and b3[2] == 0
+
+    def fwd(x=p(), xd=0, w=p(), wd=1, M=4, N=8, K=200, sv=p(), wk=p(), y=p(), yd=0, ldy=8):
+        return lib.quartet_linear_fp8_train_fwd(x, xd, w, wd, M, N, K, 1, 1, sv, wk, y, yd, ldy, None)
+
+    for name in ("x", "w", "sv", "wk", "y"):
+        assert fwd(**{name: None}) == -1
+    for name in ("sv", "wk", "y"):
+        assert fwd(**{name: p(8)}) == -3
+    assert fwd(x=p(1)) == -3 and fwd(w=p(2)) == -3 and fwd(xd=2) == -4 and fwd(wd=2) == -4 and fwd(yd=2) == -4
+    assert fwd(M=0) == -2 and fwd(N=0) == -2 and fwd(K=0) == -2 and fwd(K=8388481) == -2 and fwd(ldy=7) == -2 and fwd(ldy=12) == -2
+
+    def bwd(e=p(), ed=0, M=4, N=8, K=200, fmt=0, sv=p(), wk=p(), dx=p(), xd=0, ldx=200, dw=p(), wd=1, ldw=200, sx=1, sw=1):
+        return lib.quartet_linear_fp8_train_bwd(e, ed, M, N, K, fmt, sv, wk, dx, xd, ldx, dw, wd, ldw, sx, sw, None)
+
+    for name in ("e", "sv", "wk"):
+        assert bwd(**{name: None}) == -1
+    for name in ("sv", "wk", "dx", "dw"):
+        assert bwd(**{name: p(8)}) == -3
+    assert bwd(dx=None, dw=None, e=None) == 0 and bwd(e=p(1)) == -3
+    assert bwd(sx=0) == -4 and bwd(sw=0) == -4 and bwd(fmt=2) == -4 and bwd(ed=2) == -4 and bwd(xd=2) == -4 and bwd(wd=2) == -4
+    assert bwd(M=0) == -2 and bwd(ldx=199) == -2 and bwd(ldw=202) == -2
+
+
 def test_rotary_refusals(lib, p):
     def f(n=1, src=(p(),), dst=(p(1024),), strides=(0,) * 18, heads=(1,), rotate=(1,), dt=0, batch=1, tokens=1, d=64, rot=64, pos=None, i64=1, inv=p(2048)):
         m = max(len(src), 1)
