@@ -9,9 +9,10 @@
 // The products are m16n8k16 in fp16, which holds every 8-bit code: 16 rows of B, converted as they come from shared memory, and the
 // (up to) eight rows of A, converted once.  Sums over 32 values are scaled by their two E8M0 factors in fp32 and added to
 // fp32 sums, which the warps of a group join in a fixed order in shared memory.  (The 8-bit form of the instruction converts both operands
-// inside: 30 us at N 12288, K 4096, one row, against 17.)  Bound by the issue of instructions, about 320 for 2 KB: eight warps take 21 us.
-// us at one row, quantizer included, here / tensor-memory kernel with its quantizer: N 12288, K 4096 17.1 / 16.5; N 4096, K 11008 15.2 / 14.3; N 32000,
-// K 640 8.0 / 8.0, of which a caller pays one launch / two.
+// inside: 30 us at N 12288, K 4096, one row, where this takes 14.)  Bound by the issue of instructions before the memory: eight warps instead of
+// sixteen took half as long again, and 32 warps or deeper rings gain nothing.
+// us at one row, quantizer included, here / tensor-memory kernel behind its quantizer: N 12288, K 4096 14.1 / 15.5; N 4096, K 11008 12.6 / 13.7;
+// N 32000, K 640 7.1 / 7.7.
 // A comes as codes and scales, or as values that the CTA quantizes into shared memory while its first copies are under way.
 #include "common.cuh"
 #include "gemm_fp8.cuh"
@@ -47,6 +48,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 struct GemvParams {
@@ -86,23 +92,30 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
     pdl_launch_dependents();
     pdl_wait();
 
-    // the ring's position in this warp's sequence of (block, chunk)
-    int blk = blockIdx.x, ck = 0;
-    auto issue = [&](int s) {  // lane 0
-        const int row0 = (blk * rw + group) * 16;
-        mbar_arrive_expect_tx(&full[s], GEMV_STAGE_BYTES);
-        tma_load_2d(s_w + s * GEMV_W_BYTES, &tm_w, (c0 + ck) * 128, row0, &full[s]);
-        bulk_load(s_sf + s * GEMV_SF_BYTES, p.g.b_sf + ((int64_t)(row0 >> 7) * chunks + c0 + ck) * 512 + (row0 & 31) * 16, GEMV_SF_BYTES, &full[s]);
+    // The ring's position in this warp's sequence of (block, chunk): coordinates and the scales' address move on by addition.  Blocks whose
+    // group lies past the last row are the last ones, and are left out.
+    const int blocks_mine = (int)((p.g.N - (int64_t)group * 16 + rw * 16 - 1) / (rw * 16));     // blocks whose rows of this group exist
+    int blk = blockIdx.x, ck = 0, row0 = 0;
+    const uint8_t* sf_src = nullptr;
+    auto at_block = [&]() {
+        row0 = (blk * rw + group) * 16;
+        sf_src = p.g.b_sf + ((int64_t)(row0 >> 7) * chunks + c0) * 512 + (row0 & 31) * 16;
     };
-    // blocks whose group lies past the last row are passed over by every lane alike
-    auto skip = [&](int b) { return (int64_t)(b * rw + group) * 16 >= p.g.N; };
+    at_block();
     int ahead = 0;  // copies issued and not yet consumed
     auto fill = [&](int s) {
-        while (blk < p.blocks && skip(blk)) blk += gridDim.x;
-        if (blk >= p.blocks || mine == 0) return;
-        if (lane == 0) issue(s);
+        if (blk >= blocks_mine || mine == 0) return;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&full[s], GEMV_STAGE_BYTES);
+            tma_load_2d(s_w + s * GEMV_W_BYTES, &tm_w, (c0 + ck) * 128, row0, &full[s]);
+            bulk_load(s_sf + s * GEMV_SF_BYTES, sf_src, GEMV_SF_BYTES, &full[s]);
+        }
         ++ahead;
-        if (++ck == mine) ck = 0, blk += gridDim.x;
+        sf_src += 512;
+        if (++ck == mine) {
+            ck = 0, blk += gridDim.x;
+            at_block();
+        }
     };
     for (int s = 0; s < GEMV_STAGES; ++s) fill(s);
 
@@ -151,53 +164,55 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
     __syncthreads();
 
     const int g = lane >> 2, q = lane & 3;     // accumulator: rows g, g + 8 of B, tokens 2 q, 2 q + 1
-    const uint8_t* a_row = s_a + (g < M ? g : 0) * pitch + q * 8;
-    const uint32_t* asf0 = s_asf + (2 * q < M ? 2 * q : 0) * chunks;
-    const uint32_t* asf1 = s_asf + (2 * q + 1 < M ? 2 * q + 1 : 0) * chunks;
+    // (rows of A past the last one: the first row's values, whose results nobody reads)
+    const uint8_t* a_row = s_a + (g < M ? g : 0) * pitch + c0 * 256 + q * 8;
+    const uint32_t* asf0 = s_asf + (2 * q < M ? 2 * q : 0) * chunks + c0;
+    const uint32_t* asf1 = s_asf + (2 * q + 1 < M ? 2 * q + 1 : 0) * chunks + c0;
+    // ldmatrix: lanes 0-7 rows 0-7, 8-15 rows 8-15 of the first 16 bytes, 16-31 the same of the second; 128-byte swizzle
+    uint32_t m_off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m_off[k] = (lane & 15) * 128 + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4);
+    const uint32_t w_base = smem_u32(s_w);
     uint32_t s = 0, ph = 0, buf = 0;
     bool dead = false;                         // a wait gave up: this warp only keeps the barriers
     for (int b = blockIdx.x; b < p.blocks; b += gridDim.x, buf ^= 1) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const int row0 = (b * rw + group) * 16;
-        if (!dead && !skip(b)) {
-            const int seg = (row0 >> 5) & 3;
+        if (!dead && b < blocks_mine) {
+            const int seg = ((b * rw + group) >> 1) & 3;  // 32-row segment of the rows in their block of 128
             for (int c = 0; c < mine; ++c) {
                 if (!mbar_wait(&full[s], ph, WAIT_GEMM_FULL)) {
                     dead = true;
                     break;
                 }
                 --ahead;
-                const uint8_t* sfw = s_sf + s * GEMV_SF_BYTES + seg * 4;
-                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(sfw + g * 16), w1 = *reinterpret_cast<const uint32_t*>(sfw + (g + 8) * 16);
-                const uint32_t x0 = asf0[c0 + c], x1 = asf1[c0 + c];
-                const uint32_t base = smem_u32(s_w + s * GEMV_W_BYTES);
-                // ldmatrix: lanes 0-7 rows 0-7, 8-15 rows 8-15 of the first 16 bytes, 16-31 the same of the second
-                const int mrow = lane & 15, half = lane >> 4;
-                const uint8_t* av = a_row + (c0 + c) * 256;
-                float cc[4][4] = {};
+                const uint8_t* sfw = s_sf + s * GEMV_SF_BYTES + seg * 4 + g * 16;
+                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(sfw), w1 = *reinterpret_cast<const uint32_t*>(sfw + 128);
+                const uint32_t x0 = asf0[c], x1 = asf1[c];
+                const uint32_t base = w_base + s * GEMV_W_BYTES;
+                const uint8_t* av = a_row + c * 256;
+                float cc[4][4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     uint32_t f[4];
-                    const uint32_t addr = base + mrow * 128 + (((2 * k + half) ^ (mrow & 7)) << 4);
                     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
-                                 : "r"(addr)
+                                 : "r"(base + m_off[k])
                                  : "memory");
                     // a thread's four neighbouring values of a row stand for the instruction's columns 2 q, 2 q + 1, 2 q + 8, 2 q + 9, and so do A's
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint2 xv = *reinterpret_cast<const uint2*>(av + k * 64 + h * 32);
-                        if (g >= M) xv = make_uint2(0u, 0u);
-                        mma_f16(cc[k], f16x2_of<B_E5M2>(f[2 * h]), f16x2_of<B_E5M2>(f[2 * h + 1]), f16x2_of<B_E5M2>(f[2 * h] >> 16),
-                                f16x2_of<B_E5M2>(f[2 * h + 1] >> 16), xv.x, xv.y);
-                    }
+                    const uint2 xa = *reinterpret_cast<const uint2*>(av + k * 64), xb = *reinterpret_cast<const uint2*>(av + k * 64 + 32);
+                    mma_f16_first(cc[k], f16x2_of<B_E5M2>(f[0]), f16x2_of<B_E5M2>(f[1]), f16x2_of<B_E5M2>(f[0] >> 16), f16x2_of<B_E5M2>(f[1] >> 16), xa.x, xa.y);
+                    mma_f16(cc[k], f16x2_of<B_E5M2>(f[2]), f16x2_of<B_E5M2>(f[3]), f16x2_of<B_E5M2>(f[2] >> 16), f16x2_of<B_E5M2>(f[3] >> 16), xb.x, xb.y);
                 }
                 __syncwarp();
                 fill((int)s);  // the stage is in registers: its next copy may start
                 if (++s == GEMV_STAGES) s = 0, ph ^= 1;
-                const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0);
-                if (__all_sync(0xFFFFFFFFu, block)) {  // one scale for the whole chunk, as this library's quantizers write them
-                    const float sw0 = e8m0_value(w0 & 255u), sw1 = e8m0_value(w1 & 255u), sx0 = e8m0_value(x0 & 255u), sx1 = e8m0_value(x1 & 255u);
+                // one scale for the whole chunk, as this library's quantizers write them, and none of them NaN
+                const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0) &&
+                                   max(max(w0, w1), max(x0, x1)) < 0xFF000000u;
+                if (__all_sync(0xFFFFFFFFu, block)) {
+                    // byte b in the exponent's place; for 0 the subnormal 2^-127
+                    const float sw0 = __uint_as_float(max((w0 >> 24) << 23, 0x00400000u)), sw1 = __uint_as_float(max((w1 >> 24) << 23, 0x00400000u));
+                    const float sx0 = __uint_as_float(max((x0 >> 24) << 23, 0x00400000u)), sx1 = __uint_as_float(max((x1 >> 24) << 23, 0x00400000u));
                     acc[0] = fmaf(((cc[0][0] + cc[1][0]) + (cc[2][0] + cc[3][0])) * sw0, sx0, acc[0]);
                     acc[1] = fmaf(((cc[0][1] + cc[1][1]) + (cc[2][1] + cc[3][1])) * sw0, sx1, acc[1]);
                     acc[2] = fmaf(((cc[0][2] + cc[1][2]) + (cc[2][2] + cc[3][2])) * sw1, sx0, acc[2]);

@@ -652,10 +652,13 @@ def _dense(t) -> bool:
 
 def _tensor_list(ts, dev, what):
     """Host arrays (addresses, element counts, dtypes) of the tensors."""
-    dts = [_LIST_DT.get(t.dtype, -1) for t in ts]
-    if dev.type != "cuda" or -1 in dts or any([t.device != dev for t in ts]) or not all([t.is_contiguous() or _dense(t) for t in ts]):
+    try:
+        dts = array("i", [_LIST_DT[t.dtype] for t in ts])
+    except KeyError:
+        dts = None
+    if dts is None or dev.type != "cuda" or any([t.device != dev for t in ts]) or not all([t.is_contiguous() or _dense(t) for t in ts]):
         raise ValueError(f"{what} must be dense bf16 or fp32 tensors on one CUDA device")
-    return array("q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]), array("i", dts)
+    return array("q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]), dts
 
 
 def _at(a) -> int:
@@ -699,6 +702,7 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
     optrs, odts = ptrs, dts
     if out is not None:
         out = list(out)
+        # (strides of contiguous tensors may differ where an axis has one element; equal strides are the common case)
         if len(out) != len(tensors) or any([o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))
                                             for o, t in zip(out, tensors)]):
             raise ValueError("out must hold a tensor of the same shape and strides for each of the tensors")
