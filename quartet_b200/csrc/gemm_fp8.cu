@@ -633,9 +633,13 @@ static int launch_pair(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8G
 
 QUARTET_DEFINE_STATUS_READER(status_gemm_fp8)
 
+// Which kernel.  Up to eight rows: the stream over B.  Else CTA pairs, unless the result has so few 128 x 128 tiles that splitting the contraction
+// occupies more SMs: the longer the contraction, the more tiles that pays for (us, pairs / split: K 640, 15 tiles 6.7 / 6.1, 20 tiles
+// 6.5 / 7.2; K 4096, 64 tiles 14.6 / 13.8, 96 tiles 15.1 / 17.0).
 static int product(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t s) {
     if (gemv_fits(p.M, K)) return gemv_fp8_codes(a, b, p, s);
-    if (p.M >= 256 && p.N >= 256) return launch_pair(a, b, K, p, s);
+    const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 127) / 128), few = 8 + 2 * p.k_chunks;
+    if (p.M > 64 && p.N >= 256 && tiles > (few < 72 ? few : 72)) return launch_pair(a, b, K, p, s);
     if (p.M > 64) return launch_split<128>(a, b, K, p, s);
     return p.M > 32 ? launch_split<64>(a, b, K, p, s) : launch_split<32>(a, b, K, p, s);
 }

@@ -505,6 +505,8 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
     blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear."""
     _need_codes(w, w_sf, "linear_fp8")
     shape, dev = x.shape, w.device
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError("x must have at least one column")
     K, N = shape[-1], w.shape[0]
     if (K + 127) // 128 * 128 != w.shape[1]:
         raise ValueError(f"x has {K} columns, the weight {w.shape[1]}")

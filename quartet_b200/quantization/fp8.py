@@ -48,7 +48,7 @@ class _Fp8LinearFn(torch.autograd.Function):
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, grad_dtype: torch.dtype = torch.float8_e4m3fn, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., K] (bf16 / fp32) times weight [N, K]^T on 8-bit operands, differentiable in both.  out_dtype: bf16 or fp32; by default autocast's, else
     x's.  For a weight that does not change, pack it once (ops.quant_fp8(weight, square=True)) and call ops.linear_fp8."""
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"x [..., K] and weight [N, K] are needed, not {tuple(x.shape)} and {tuple(weight.shape)}")
     if not (x.is_cuda and weight.device == x.device):
         raise ValueError("x and weight must live on one CUDA device")

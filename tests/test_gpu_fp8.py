@@ -118,7 +118,8 @@ def _product(ops, M, N, K, fa=E4M3, fb=E4M3, out_dtype=torch.float32, seed=0, al
 
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 257, 640), (5, 130, 127), (16, 512, 1024), (17, 96, 384), (33, 640, 129), (64, 1000, 512), (65, 264, 2048), (100, 100, 100),
          (128, 128, 4096), (129, 255, 640), (250, 1024, 300), (256, 256, 256), (257, 513, 1152), (384, 128, 1408), (511, 264, 520), (1021, 640, 640),
-         (1024, 2051, 256), (2048, 520, 384)]
+         (1024, 2051, 256), (2048, 520, 384),
+         (65, 4099, 128), (96, 4096, 640), (200, 2300, 256), (255, 3000, 384), (300, 257, 8192), (2000, 256, 128)]
 
 
 @pytest.mark.parametrize("mnk", SIZES)
@@ -341,6 +342,6 @@ def test_refusals(ops):
                  lambda: ops.quant_fp8(x.cpu()), lambda: ops.quant_fp8(x[0]), lambda: ops.gemm_fp8_tn(c, sf, c[:, :128].contiguous(), sf),
                  lambda: ops.gemm_fp8_tn(c, sf[:-1], c, sf), lambda: ops.gemm_fp8_tn(c.view(torch.uint8), sf, c, sf),
                  lambda: ops.gemm_fp8_tn(c, sf, c, sf, out_dtype=torch.float16), lambda: ops.linear_fp8(x[:, :100], c, sf), lambda: ops.dequant_fp8(c, sf, 100),
-                 lambda: fp8_linear(x, x[:, :128]), lambda: fp8_linear(x.cpu(), x), lambda: fp8_linear(x, x, grad_dtype=torch.int8)):
+                 lambda: fp8_linear(x, x[:, :128]), lambda: fp8_linear(x[:, :0], x[:, :0]), lambda: ops.linear_fp8(x[:, :0], c, sf), lambda: fp8_linear(x.cpu(), x), lambda: fp8_linear(x, x, grad_dtype=torch.int8)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
