@@ -585,7 +585,7 @@ def rotary(segments, inv_freq, positions=None, offset=0, interleaved=True, scale
     x0 = segments[0][0]
     B, T, _, d = x0.shape
     dev, dtype = x0.device, x0.dtype
-    ptrs, strides, heads = [], [], []
+    srcs, dsts, strides, heads, turns = [], [], [], [], []
     for src, dst, rotate in segments:
         shape = src.shape
         if src.device != dev or dst.device != dev:
@@ -595,16 +595,22 @@ def rotary(segments, inv_freq, positions=None, offset=0, interleaved=True, scale
         a, b = src.stride(), dst.stride()
         if d > 1 and (a[3] != 1 or b[3] != 1):
             raise ValueError("the values of a head must be adjacent")
-        ptrs.append((src.data_ptr(), dst.data_ptr()))
+        srcs.append(src.data_ptr()), dsts.append(dst.data_ptr()), heads.append(shape[2]), turns.append(1 if rotate else 0)
         strides += [a[0], a[1], a[2], b[0], b[1], b[2]]
-        heads.append((shape[2], 1 if rotate else 0))
-    rotary_raw(ptrs, strides, heads, dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse)
+    rotary_raw(srcs + dsts, rotary_plan(strides, heads, turns), dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse)
 
 
-def rotary_raw(ptrs, strides, heads, dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse):
-    """The launch behind rotary(): ptrs [(src, dst)], strides six integers a segment (batch, token, head of src and dst), heads [(count, rotate)]
-    of segments that the caller has checked; inv_freq and positions are checked here."""
-    n = len(ptrs)
+def rotary_plan(strides, heads, turns):
+    """The host arrays of a launch that do not change with the tensors' addresses: element strides (batch, token, head of src and dst) of each
+    segment, its heads and whether it is turned."""
+    longs, ints = array("q", strides), array("i", [*heads, *turns])
+    return longs, ints, longs.buffer_info()[0], ints.buffer_info()[0]
+
+
+def rotary_raw(ptrs, plan, dev, dtype, B, T, d, inv_freq, positions, offset, interleaved, scale, inverse):
+    """The launch behind rotary(): ptrs (sources, then destinations) and plan (rotary_plan) of segments that the caller has checked; inv_freq and
+    positions are checked here."""
+    n = len(ptrs) >> 1
     if dev.type != "cuda":
         raise ValueError("tensors must live on a CUDA device")
     if inv_freq.device != dev or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
@@ -624,12 +630,11 @@ def rotary_raw(ptrs, strides, heads, dev, dtype, B, T, d, inv_freq, positions, o
         raise ValueError(f"dtype {dtype} not supported (bf16 or fp32)")
     if B * T == 0:
         return
-    longs = array("q", [a for a, _ in ptrs] + [b for _, b in ptrs] + strides)
-    ints = array("i", [h for h, _ in heads] + [r for _, r in heads])
-    at, it = longs.buffer_info()[0], ints.buffer_info()[0]
+    addresses = array("q", ptrs)
+    at, (_, _, strides, ints) = addresses.buffer_info()[0], plan
     with _on(dev):
-        rc = _lib.load().quartet_rotary(n, at, at + 8 * n, at + 16 * n, it, it + 4 * n, _LIST_DT[dtype], B, T, d, 2 * inv_freq.numel(),
-                                        1 if interleaved else 0, pos_ptr, i64, pb, pt, offset, inv_freq.data_ptr(), scale, 1 if inverse else 0, _stream())
+        rc = _lib.load().quartet_rotary(n, at, at + 8 * n, strides, ints, ints + 4 * n, _LIST_DT[dtype], B, T, d, 2 * inv_freq.shape[0], 1 if interleaved else 0,
+                                        pos_ptr, i64, pb, pt, offset, inv_freq.data_ptr(), scale, 1 if inverse else 0, _stream())
     if rc:
         _lib.check(rc, "quartet_rotary")
 

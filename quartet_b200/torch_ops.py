@@ -19,6 +19,7 @@ implementation behind these operators.
 """
 from __future__ import annotations
 
+import functools
 import random
 import weakref
 from typing import Optional, Tuple
@@ -424,45 +425,58 @@ torch.library.register_autograd("quartet_b200::swiglu_linear_fwd", _swiglu_linea
 # ------------------------------------------------------------------------------------------------
 # rotary positions
 # ------------------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=1024)
+def _qkv_plan(hq: int, hk: int, t: int, d: int, sb: int, st: int, head_major: bool, join: bool):
+    """rotary_plan of a packed projection with strides (sb, st) and contiguous heads, in the one direction or the other."""
+    strides = []
+    for h in (hq, hk, hk):
+        packed, heads = [sb, st, d], ([h * t * d, d, t * d] if head_major else [t * h * d, h * d, d])
+        strides += heads + packed if join else packed + heads
+    return ops.rotary_plan(strides, (hq, hk, hk), (1, 1, 0))
+
+
 def split_heads(qkv: Tensor, n_head: int, n_kv_head: int, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
                 head_major: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """Packed projection -> q, k (turned) and v in one launch.  Addresses and strides are worked out here: a view of torch's costs more
     than the launch."""
-    if qkv.stride(2) != 1:
-        qkv = qkv.contiguous()
     b, t, w = qkv.shape
+    sb, st, s1 = qkv.stride()
+    if s1 != 1:
+        qkv = qkv.contiguous()
+        sb, st, _ = qkv.stride()
     d = w // (n_head + 2 * n_kv_head)
-    sb, st, _ = qkv.stride()
-    q = qkv.new_empty((b, n_head, t, d) if head_major else (b, t, n_head, d))
-    k, v = (qkv.new_empty((b, n_kv_head, t, d) if head_major else (b, t, n_kv_head, d)) for _ in range(2))
-    src, es = qkv.data_ptr(), qkv.element_size()
-    ptrs = [(src, q.data_ptr()), (src + n_head * d * es, k.data_ptr()), (src + (n_head + n_kv_head) * d * es, v.data_ptr())]
-    strides = []
-    for h in (n_head, n_kv_head, n_kv_head):
-        strides += [sb, st, d, h * t * d, d, t * d] if head_major else [sb, st, d, t * h * d, h * d, d]
-    ops.rotary_raw(ptrs, strides, [(n_head, 1), (n_kv_head, 1), (n_kv_head, 0)], qkv.device, qkv.dtype, b, t, d, inv_freq, positions, offset, interleaved, scale,
-                   False)
+    dev, dtype = qkv.device, qkv.dtype
+    kv = (b, n_kv_head, t, d) if head_major else (b, t, n_kv_head, d)
+    q, k, v = qkv.new_empty((b, n_head, t, d) if head_major else (b, t, n_head, d)), qkv.new_empty(kv), qkv.new_empty(kv)
+    src, row = qkv.data_ptr(), d * qkv.element_size()
+    ops.rotary_raw((src, src + n_head * row, src + (n_head + n_kv_head) * row, q.data_ptr(), k.data_ptr(), v.data_ptr()),
+                   _qkv_plan(n_head, n_kv_head, t, d, sb, st, head_major, False), dev, dtype, b, t, d, inv_freq, positions, offset, interleaved, scale, False)
     return q, k, v
 
 
 def join_heads(dq: Tensor, dk: Tensor, dv: Tensor, inv_freq: Tensor, positions: Optional[Tensor], offset: int, interleaved: bool, scale: float,
                head_major: bool) -> Tensor:
     """The gradient of split_heads: gradients of q, k, v (any strides) -> the packed one."""
-    gs = [g if g.stride(3) == 1 else g.contiguous() for g in (dq, dk, dv)]
-    ax_t, ax_h = (2, 1) if head_major else (1, 2)
-    b, t, d = dq.shape[0], dq.shape[ax_t], dq.shape[3]
-    heads = [g.shape[ax_h] for g in gs]
-    w = sum(heads) * d
+    if head_major:
+        b, hq, t, d = dq.shape
+        hk = dk.shape[1]
+    else:
+        b, t, hq, d = dq.shape
+        hk = dk.shape[2]
+    w = (hq + 2 * hk) * d
     out = dq.new_empty((b, t, w))
-    dst, es = out.data_ptr(), out.element_size()
-    ptrs, strides = [], []
-    for g, h in zip(gs, heads):
-        st = g.stride()
-        ptrs.append((g.data_ptr(), dst))
-        strides += [st[0], st[ax_t], st[ax_h], t * w, w, d]
-        dst += h * d * es
-    ops.rotary_raw(ptrs, strides, [(heads[0], 1), (heads[1], 1), (heads[2], 0)], out.device, out.dtype, b, t, d, inv_freq, positions, offset, interleaved, scale,
-                   True)
+    if dq.is_contiguous() and dk.is_contiguous() and dv.is_contiguous():
+        plan = _qkv_plan(hq, hk, t, d, t * w, w, head_major, True)
+    else:
+        dq, dk, dv = (g if g.stride(3) == 1 else g.contiguous() for g in (dq, dk, dv))
+        strides = []
+        for g in (dq, dk, dv):
+            s0, s1, s2, _ = g.stride()
+            strides += [s0, s2, s1, t * w, w, d] if head_major else [s0, s1, s2, t * w, w, d]
+        plan = ops.rotary_plan(strides, (hq, hk, hk), (1, 1, 0))
+    dst, row = out.data_ptr(), d * out.element_size()
+    ops.rotary_raw((dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dst, dst + hq * row, dst + (hq + hk) * row), plan, out.device, out.dtype, b, t, d, inv_freq,
+                   positions, offset, interleaved, scale, True)
     return out
 
 
