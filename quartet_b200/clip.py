@@ -14,9 +14,11 @@ from . import ops
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, group=None) -> torch.Tensor:
     """Scales the gradients in place so that their norm (2 or inf) is at most max_norm; returns the norm before, fp32, on the device.
 
-    A parameter with a `grad_shard` and no `grad` counts as sharded: the squares of shards are summed over the ranks of `group`
-    (every rank then has to make this call); gradients in `.grad` are taken to be the same on every rank.
+    Gradients are dense bf16 or fp32 tensors on one device.  A parameter with a `grad_shard` and no `grad` counts as sharded: the norm is
+    taken over the shards of all ranks of `group` (every rank then has to make this call); gradients in `.grad` are taken to be the
+    same on every rank.
     error_if_nonfinite reads the norm back, and raises before anything is scaled."""
+    norm_type = float(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     whole = [p.grad for p in parameters if p.grad is not None]
     shards = [p.grad_shard for p in parameters if p.grad is None and getattr(p, "grad_shard", None) is not None]
@@ -28,7 +30,13 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         if not dist.is_initialized():
             raise RuntimeError("sharded gradients need an initialised process group")
         total = ops.grad_norm(shards, norm_type, total=True)
-        dist.all_reduce(total, op=dist.ReduceOp.MAX if norm_type == float("inf") else dist.ReduceOp.SUM, group=group)
+        if norm_type == float("inf"):
+            # gathered, not reduced: a library's maximum may drop a NaN, torch's does not
+            every = [torch.empty_like(total) for _ in range(dist.get_world_size(group))]
+            dist.all_gather(every, total, group=group)
+            total = torch.cat(every).max().reshape(1)
+        else:
+            dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
         if whole:
             rest = ops.grad_norm(whole, norm_type, total=True)
             total = torch.maximum(total, rest) if norm_type == float("inf") else total + rest

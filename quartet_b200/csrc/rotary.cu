@@ -44,13 +44,14 @@ template <bool F32, bool VEC>
 struct RotVec {
     static constexpr int N = VEC ? (F32 ? 4 : 8) : 1;
     uint4 q;
+    // (plain loads, not read-only ones: a tensor may be turned in place)
     __device__ __forceinline__ void load(const void* p, int64_t i) {
         if constexpr (VEC)
-            q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (F32 ? 4 : 2)));
+            q = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (F32 ? 4 : 2));
         else if constexpr (F32)
-            q.x = __ldg(static_cast<const uint32_t*>(p) + i);
+            q.x = static_cast<const uint32_t*>(p)[i];
         else
-            q.x = (uint32_t)__ldg(static_cast<const uint16_t*>(p) + i) << 16;
+            q.x = (uint32_t)static_cast<const uint16_t*>(p)[i] << 16;
     }
     __device__ __forceinline__ void copy(void* p, int64_t i) const {
         if constexpr (VEC)

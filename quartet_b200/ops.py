@@ -673,6 +673,7 @@ def _at(a) -> int:
 
 
 def _norm_kind(norm_type) -> int:
+    norm_type = float(norm_type)
     if norm_type == 2:
         return 0
     if norm_type == float("inf"):

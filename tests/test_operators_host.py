@@ -207,7 +207,7 @@ def test_frequencies():
             rotary_frequencies(bad)
 
 
-def _shard_rank(rank, port, inf, out):
+def _shard_rank(rank, port, inf, nan, out):
     import torch.distributed as dist
 
     from quartet_b200 import clip, ops
@@ -222,7 +222,7 @@ def _shard_rank(rank, port, inf, out):
     def scale(ts, max_norm, kind=2.0, out=None, total=None):
         n = total[0] if kind == math.inf else total[0].sqrt()
         for t in ts:
-            t.mul_(float(min(1.0, max_norm / (n + 1e-6))))
+            t.mul_(float((max_norm / (n + 1e-6)).clamp(max=1.0)))
         return n.float()
 
     ops.grad_norm, ops.clip_grads = total_of, scale
@@ -230,16 +230,20 @@ def _shard_rank(rank, port, inf, out):
     full, rest = torch.randn(8, 5, generator=g), torch.randn(7, generator=g)
     p, q = torch.nn.Parameter(torch.zeros(8, 5)), torch.nn.Parameter(torch.zeros(7))
     p.grad_shard, q.grad = full[4 * rank:4 * rank + 4].clone(), rest.clone()
+    if nan and rank == 1:
+        p.grad_shard[2, 3] = math.nan
     n = clip.clip_grad_norm_([p, q], 0.5, math.inf if inf else 2.0)
     both = torch.cat([full.reshape(-1), rest]).double()
     want = both.abs().max() if inf else both.norm()
     ok = abs(n.item() - want.item()) < 1e-6 and torch.allclose(p.grad_shard, full[4 * rank:4 * rank + 4] * (0.5 / want).float(), rtol=1e-5)
-    out[rank] = ok and torch.allclose(q.grad, rest * (0.5 / want).float(), rtol=1e-5)
+    if nan:
+        ok = math.isnan(n.item()) and bool(torch.isnan(p.grad_shard).all()) and bool(torch.isnan(q.grad).all())
+    out[rank] = ok if nan else ok and torch.allclose(q.grad, rest * (0.5 / want).float(), rtol=1e-5)
     dist.destroy_process_group()
 
 
-@pytest.mark.parametrize("inf", [False, True])
-def test_sharded_clip_over_two_ranks(inf):
+@pytest.mark.parametrize("inf,nan", [(False, False), (True, False), (False, True), (True, True)])
+def test_sharded_clip_over_two_ranks(inf, nan):
     import socket
 
     import torch.multiprocessing as mp
@@ -250,7 +254,7 @@ def test_sharded_clip_over_two_ranks(inf):
     ctx = mp.get_context("spawn")
     with ctx.Manager() as m:
         out = m.dict()
-        mp.spawn(_shard_rank, args=(port, inf, out), nprocs=2)
+        mp.spawn(_shard_rank, args=(port, inf, nan, out), nprocs=2)
         assert dict(out) == {0: True, 1: True}
 
 
