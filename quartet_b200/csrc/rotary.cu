@@ -8,9 +8,9 @@
 //
 // Angles: the turn pos * inv_freq / 2 pi is taken in 64 bits and reduced there, because in 32 bits a position of 2^17 leaves an angle
 // 2^-7 wrong; its fraction goes to sincospif, with the part that 32 bits lose put back to first order.  They cost no memory traffic
-// and no table in it: a thread owns the same few pairs of a token in all heads, computes their sines and cosines once, keeps them in
-// registers and walks the heads, four at a time.  Where there are few tokens a thread takes every split-th head, and the threads of a token
-// share its pairs through shared memory.
+// and no table in it: a thread owns the same few pairs of a token in all heads of all segments, computes their sines and cosines once, keeps
+// them in registers and walks the heads in batches, the next batch's loads under way while one is turned and stored.  Where there are few
+// tokens a thread takes every split-th head, and the threads of a token share its pairs through shared memory.
 // Bound by memory: each value is read and written once.
 #include "common.cuh"
 #include "quant_math.cuh"
@@ -45,21 +45,21 @@ struct RotVec {
     static constexpr int N = VEC ? (F32 ? 4 : 8) : 1;
     uint4 q;
     // (plain loads, not read-only ones: a tensor may be turned in place)
-    __device__ __forceinline__ void load(const void* p, int64_t i) {
+    __device__ __forceinline__ void load(const uint8_t* p) {
         if constexpr (VEC)
-            q = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (F32 ? 4 : 2));
+            q = *reinterpret_cast<const uint4*>(p);
         else if constexpr (F32)
-            q.x = static_cast<const uint32_t*>(p)[i];
+            q.x = *reinterpret_cast<const uint32_t*>(p);
         else
-            q.x = (uint32_t)static_cast<const uint16_t*>(p)[i] << 16;
+            q.x = (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16;
     }
-    __device__ __forceinline__ void copy(void* p, int64_t i) const {
+    __device__ __forceinline__ void copy(uint8_t* p) const {
         if constexpr (VEC)
-            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * (F32 ? 4 : 2)) = q;
+            *reinterpret_cast<uint4*>(p) = q;
         else if constexpr (F32)
-            static_cast<uint32_t*>(p)[i] = q.x;
+            *reinterpret_cast<uint32_t*>(p) = q.x;
         else
-            static_cast<uint16_t*>(p)[i] = (uint16_t)(q.x >> 16);
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)(q.x >> 16);
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {
         if constexpr (VEC && !F32) {
@@ -70,9 +70,9 @@ struct RotVec {
             for (int k = 0; k < N; ++k) v[k] = __uint_as_float(r[k]);
         }
     }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[N]) {
+    static __device__ __forceinline__ void store(uint8_t* p, const float (&v)[N]) {
         if constexpr (VEC && F32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         } else if constexpr (VEC) {
             uint32_t w[4];
 #pragma unroll
@@ -80,11 +80,11 @@ struct RotVec {
                 const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
                 w[k] = *reinterpret_cast<const uint32_t*>(&t);
             }
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
         } else if constexpr (F32) {
-            static_cast<float*>(p)[i] = v[0];
+            *reinterpret_cast<float*>(p) = v[0];
         } else {
-            static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v[0]);
+            *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v[0]);
         }
     }
 };
@@ -108,15 +108,14 @@ __device__ __forceinline__ float2 rotation(const RotParams& p, int64_t pos, int 
 template <bool F32, bool INTERLEAVED, bool VEC, bool SPLIT>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotParams p) {
     using V = RotVec<F32, VEC>;
-    // a unit is what a thread moves at once: one vector of side-by-side pairs, two vectors half a rotated part apart (two single
-    // values, in either layout), or one vector that is only copied
+    // A unit is what a thread moves of every head: one vector of side-by-side pairs, two vectors half a rotated part apart (two single
+    // values, in either layout), or one vector that is only copied.  The units cover a head, so a segment that is not turned (v) is
+    // copied by the same units.
     constexpr bool ONE = INTERLEAVED && VEC;
-    constexpr int RU = ONE ? V::N : 2 * V::N, PAIRS = RU / 2;
-    const int ru = p.rot / RU, units = ru + (p.d - p.rot) / V::N;
-    // Heads in flight.  Many tokens: four (two, for the layout with two vectors a unit: 75 us against 56 at 32768 tokens of 15 heads).  Few
-    // tokens leave a thread few heads, and registers are worth more as resident threads: 3063 tokens of 12 fp32 heads 10.3 us with four, 7.3 with two.
-    constexpr int ROT_AHEAD = SPLIT ? 2 : 4;
+    constexpr int RU = ONE ? V::N : 2 * V::N, PAIRS = RU / 2, ES = F32 ? 4 : 2;
+    constexpr int BATCH = SPLIT ? 1 : ONE ? 4 : 2;  // heads: 64 bytes a batch
     extern __shared__ __align__(16) float2 s_cs[];  // [token of the block][pair]
+    const int ru = p.rot / RU, units = ru + (p.d - p.rot) / V::N;
     const int lane = threadIdx.x % p.lanes, rest = threadIdx.x / p.lanes, group = rest % p.split, mine = rest / p.split;
     const int pairs = p.rot >> 1;
     const int64_t token = (int64_t)blockIdx.x * p.per_block + mine;
@@ -131,14 +130,34 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_consta
         __syncthreads();
     }
     if (token >= p.tokens) return;
-    const int64_t pos = SPLIT ? 0 : position(p, token);
     const int64_t b = (uint32_t)token / (uint32_t)p.T, t = token - b * p.T;
     for (int i = lane; i < units; i += p.lanes) {
-        const bool turns = i < ru;
+        const bool turns = i < ru, two = !ONE && turns;
         const int a1 = !turns ? p.rot + (i - ru) * V::N : ONE ? i * RU : (INTERLEAVED ? 2 * i : i * V::N);
-        const int a2 = INTERLEAVED ? a1 + 1 : a1 + (p.rot >> 1);  // (second vector of a unit that has two)
+        const int64_t gap = (int64_t)(INTERLEAVED ? 1 : p.rot >> 1) * ES;   // from the unit's first vector to its second
+        const int64_t step = p.split;
+        auto load = [&](V (&x1)[BATCH], V (&x2)[BATCH], int g, int h) {
+            const RotSeg& sg = p.seg[g];
+            const uint8_t* src = static_cast<const uint8_t*>(sg.src) + (b * sg.s_b + t * sg.s_t + h * sg.s_h + a1) * ES;
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                if (h + u * step < sg.heads) {
+                    x1[u].load(src);
+                    if (two) x2[u].load(src + gap);
+                }
+                src += step * sg.s_h * ES;
+            }
+        };
+        auto next = [&](int& g, int& h) {
+            while (g < p.n_seg && h >= p.seg[g].heads) ++g, h = group;
+        };
+        V x1[BATCH], x2[BATCH], y1[BATCH], y2[BATCH];
+        int g = 0, h = group;
+        next(g, h);
+        if (g < p.n_seg) load(x1, x2, g, h);
         float cs[PAIRS], sn[PAIRS];
         if (turns) {
+            const int64_t pos = SPLIT ? 0 : position(p, token);
 #pragma unroll
             for (int k = 0; k < PAIRS; ++k) {
                 const float2 v = SPLIT ? s_cs[mine * pairs + i * PAIRS + k] : rotation(p, pos, i * PAIRS + k);
@@ -146,61 +165,45 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_consta
             }
         }
 #pragma unroll 1
-        for (int g = 0; g < p.n_seg; ++g) {
+        while (g < p.n_seg) {
+            int g2 = g, h2 = h + BATCH * p.split;
+            next(g2, h2);
+            if (g2 < p.n_seg) load(y1, y2, g2, h2);
             const RotSeg& sg = p.seg[g];
-            const int64_t so = b * sg.s_b + t * sg.s_t, to = b * sg.d_b + t * sg.d_t;
-            if (!sg.rotate || !turns) {
-                // copied: the vector past the rotated part, or (v) this thread's share of whole heads
-                const int first = sg.rotate ? a1 : i * V::N, last = sg.rotate ? a1 + 1 : p.d, step = units * V::N;
-                for (int at = first; at < last; at += step) {
-#pragma unroll 1
-                    for (int h0 = group; h0 < sg.heads; h0 += ROT_AHEAD * p.split) {
-                        V x[ROT_AHEAD];
+            uint8_t* dst = static_cast<uint8_t*>(sg.dst) + (b * sg.d_b + t * sg.d_t + h * sg.d_h + a1) * ES;
+            const bool turn = turns && sg.rotate;
 #pragma unroll
-                        for (int u = 0; u < ROT_AHEAD; ++u)
-                            if (h0 + u * p.split < sg.heads) x[u].load(sg.src, so + (h0 + u * p.split) * sg.s_h + at);
+            for (int u = 0; u < BATCH; ++u) {
+                if (h + u * step < sg.heads) {
+                    if (!turn) {
+                        x1[u].copy(dst);
+                        if (two) x2[u].copy(dst + gap);
+                    } else if constexpr (ONE) {
+                        float v[V::N], w[V::N];
+                        x1[u].get(v);
 #pragma unroll
-                        for (int u = 0; u < ROT_AHEAD; ++u)
-                            if (h0 + u * p.split < sg.heads) x[u].copy(sg.dst, to + (h0 + u * p.split) * sg.d_h + at);
+                        for (int k = 0; k < PAIRS; ++k) {
+                            w[2 * k] = v[2 * k] * cs[k] - v[2 * k + 1] * sn[k];
+                            w[2 * k + 1] = v[2 * k] * sn[k] + v[2 * k + 1] * cs[k];
+                        }
+                        V::store(dst, w);
+                    } else {
+                        float v1[V::N], v2[V::N], w1[V::N], w2[V::N];
+                        x1[u].get(v1);
+                        x2[u].get(v2);
+#pragma unroll
+                        for (int k = 0; k < PAIRS; ++k) {
+                            w1[k] = v1[k] * cs[k] - v2[k] * sn[k];
+                            w2[k] = v1[k] * sn[k] + v2[k] * cs[k];
+                        }
+                        V::store(dst, w1);
+                        V::store(dst + gap, w2);
                     }
                 }
-                continue;
+                dst += step * sg.d_h * ES;
+                x1[u] = y1[u], x2[u] = y2[u];
             }
-#pragma unroll 1
-            for (int h0 = group; h0 < sg.heads; h0 += ROT_AHEAD * p.split) {
-                V x1[ROT_AHEAD], x2[ROT_AHEAD];
-#pragma unroll
-                for (int u = 0; u < ROT_AHEAD; ++u)
-                    if (h0 + u * p.split < sg.heads) {
-                        const int64_t at = so + (h0 + u * p.split) * sg.s_h;
-                        x1[u].load(sg.src, at + a1);
-                        if (!ONE) x2[u].load(sg.src, at + a2);
-                    }
-#pragma unroll
-                for (int u = 0; u < ROT_AHEAD; ++u)
-                    if (h0 + u * p.split < sg.heads) {
-                        const int64_t at = to + (h0 + u * p.split) * sg.d_h;
-                        float v1[V::N], y1[V::N];
-                        x1[u].get(v1);
-                        if constexpr (ONE) {
-#pragma unroll
-                            for (int k = 0; k < PAIRS; ++k) {
-                                y1[2 * k] = v1[2 * k] * cs[k] - v1[2 * k + 1] * sn[k];
-                                y1[2 * k + 1] = v1[2 * k] * sn[k] + v1[2 * k + 1] * cs[k];
-                            }
-                        } else {
-                            float v2[V::N], y2[V::N];
-                            x2[u].get(v2);
-#pragma unroll
-                            for (int k = 0; k < PAIRS; ++k) {
-                                y1[k] = v1[k] * cs[k] - v2[k] * sn[k];
-                                y2[k] = v1[k] * sn[k] + v2[k] * cs[k];
-                            }
-                            V::store(sg.dst, at + a2, y2);
-                        }
-                        V::store(sg.dst, at + a1, y1);
-                    }
-            }
+            g = g2, h = h2;
         }
     }
 }
@@ -216,10 +219,10 @@ static int launch_rotary(RotParams p, bool interleaved, bool vec, cudaStream_t s
     const int units = p.rot / ru + (p.d - p.rot) / n;
     p.lanes = units < ROT_THREADS ? units : ROT_THREADS;
     for (int g = 0; g < p.n_seg; ++g) heads = p.seg[g].heads > heads ? p.seg[g].heads : heads;
-    // Head groups: one, so that a pair's sine and cosine are computed once, unless the threads would then be fewer than fill the GPU (a new
-    // token of each sequence).
+    // Head groups: one, so that a pair's sine and cosine are computed once by one thread, unless the threads would then be fewer than 256 an SM (a
+    // new token of each sequence; 3063 tokens of 12 fp32 heads 5.9 us with two groups, 7.7 with eight, 6.3 with one).
     p.split = 1;
-    while (p.split < heads && 2 * p.split * p.lanes <= ROT_THREADS && p.tokens * p.split * p.lanes < (int64_t)sms * 1024) p.split *= 2;
+    while (p.split < heads && 2 * p.split * p.lanes <= ROT_THREADS && p.tokens * p.split * p.lanes < (int64_t)sms * 256) p.split *= 2;
     p.per_block = ROT_THREADS / (p.lanes * p.split);
     const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
     void (*const kerns[2][2][2])(const RotParams) = {
