@@ -659,11 +659,12 @@ def _dense(t) -> bool:
 
 def _tensor_list(ts, dev, what):
     """Host arrays (addresses, element counts, dtypes) of the tensors."""
+    idx = dev.index
     try:
         dts = array("i", [_LIST_DT[t.dtype] for t in ts])
     except KeyError:
         dts = None
-    if dts is None or dev.type != "cuda" or any([t.device != dev for t in ts]) or not all([t.is_contiguous() or _dense(t) for t in ts]):
+    if dts is None or dev.type != "cuda" or any([t.get_device() != idx for t in ts]) or not all([t.is_contiguous() or _dense(t) for t in ts]):
         raise ValueError(f"{what} must be dense bf16 or fp32 tensors on one CUDA device")
     return array("q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]), dts
 
@@ -699,7 +700,7 @@ def grad_norm(tensors, norm_type=2.0, total=False):
 
 
 def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
-    """Scales the tensors by min(1, max_norm / (norm + 1e-6)), in place or into `out` (a tensor for each, fp32 or bf16, of its shape and strides);
+    """Scales the tensors by min(1, max_norm / (norm + 1e-6)), in place or into `out` (a tensor for each, fp32 or bf16, of its size and layout);
     returns the norm before (fp32 scalar on the device; nothing waits for it).  total: a float64 [1] as grad_norm(..., total=True) returns it, e.g.
     summed over ranks, to use in place of the tensors' own."""
     tensors, kind = list(tensors), _norm_kind(norm_type)
@@ -710,11 +711,11 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
     optrs, odts = ptrs, dts
     if out is not None:
         out = list(out)
-        # (strides of contiguous tensors may differ where an axis has one element; equal strides are the common case)
-        if len(out) != len(tensors) or any([o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))
-                                            for o, t in zip(out, tensors)]):
-            raise ValueError("out must hold a tensor of the same shape and strides for each of the tensors")
-        optrs, _, odts = _tensor_list(out, dev, "out")
+        optrs, onumels, odts = _tensor_list(out, dev, "out")
+        # contiguous tensors of one size lie alike in memory; others have to agree in shape and strides
+        if onumels != numels or not all([(o.is_contiguous() and t.is_contiguous()) or (o.shape == t.shape and o.stride() == t.stride())
+                                         for o, t in zip(out, tensors)]):
+            raise ValueError("out must hold a tensor of the same size and layout for each of the tensors")
     if total is not None and not (total.is_cuda and total.device == dev and total.dtype == torch.float64 and total.numel() == 1):
         raise ValueError("total must be one float64 value on the tensors' device")
     work = torch.empty(NORM_PARTIALS, dtype=torch.float64, device=dev) if total is None else None
