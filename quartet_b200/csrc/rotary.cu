@@ -39,53 +39,60 @@ struct RotParams {
     int lanes, split, per_block;  // threads a token and head group, head groups, tokens of a block
 };
 
-// Values one thread moves at a time: 16 bytes where every row allows it, single values otherwise.
-template <bool F32, bool VEC>
+// Values one thread moves at a time: as many bytes (16, 8, 4, or a single value) as every row and every half of a row allows.
+template <bool F32, int BYTES>
 struct RotVec {
-    static constexpr int N = VEC ? (F32 ? 4 : 8) : 1;
-    uint4 q;
+    static constexpr int N = BYTES / (F32 ? 4 : 2), WORDS = BYTES < 4 ? 1 : BYTES / 4;
+    uint32_t q[WORDS];
     // (plain loads, not read-only ones: a tensor may be turned in place)
     __device__ __forceinline__ void load(const uint8_t* p) {
-        if constexpr (VEC)
-            q = *reinterpret_cast<const uint4*>(p);
-        else if constexpr (F32)
-            q.x = *reinterpret_cast<const uint32_t*>(p);
-        else
-            q.x = (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16;
+        if constexpr (BYTES == 16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w;
+        } else if constexpr (BYTES == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            q[0] = v.x, q[1] = v.y;
+        } else if constexpr (BYTES == 4) {
+            q[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            q[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
     }
     __device__ __forceinline__ void copy(uint8_t* p) const {
-        if constexpr (VEC)
-            *reinterpret_cast<uint4*>(p) = q;
-        else if constexpr (F32)
-            *reinterpret_cast<uint32_t*>(p) = q.x;
+        if constexpr (BYTES == 16)
+            *reinterpret_cast<uint4*>(p) = make_uint4(q[0], q[1], q[2], q[3]);
+        else if constexpr (BYTES == 8)
+            *reinterpret_cast<uint2*>(p) = make_uint2(q[0], q[1]);
+        else if constexpr (BYTES == 4)
+            *reinterpret_cast<uint32_t*>(p) = q[0];
         else
-            *reinterpret_cast<uint16_t*>(p) = (uint16_t)(q.x >> 16);
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)q[0];
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {
-        if constexpr (VEC && !F32) {
-            unpack_bf16x8(q, v);
-        } else {
-            const uint32_t r[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = __uint_as_float(r[k]);
+        for (int k = 0; k < WORDS; ++k) {
+            if constexpr (F32) {
+                v[k] = __uint_as_float(q[k]);
+            } else {
+                v[N == 1 ? 0 : 2 * k] = __uint_as_float(q[k] << 16);
+                if constexpr (N > 1) v[2 * k + 1] = __uint_as_float(q[k] & 0xFFFF0000u);
+            }
         }
     }
     static __device__ __forceinline__ void store(uint8_t* p, const float (&v)[N]) {
-        if constexpr (VEC && F32) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        } else if constexpr (VEC) {
-            uint32_t w[4];
+        RotVec r;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < WORDS; ++k) {
+            if constexpr (F32) {
+                r.q[k] = __float_as_uint(v[k]);
+            } else if constexpr (N == 1) {
+                r.q[k] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+            } else {
                 const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-                w[k] = *reinterpret_cast<const uint32_t*>(&t);
+                r.q[k] = *reinterpret_cast<const uint32_t*>(&t);
             }
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else if constexpr (F32) {
-            *reinterpret_cast<float*>(p) = v[0];
-        } else {
-            *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v[0]);
         }
+        r.copy(p);
     }
 };
 
@@ -105,13 +112,13 @@ __device__ __forceinline__ float2 rotation(const RotParams& p, int64_t pos, int 
     return make_float2((c - s * lo) * p.scale, (s + c * lo) * (p.inverse ? -p.scale : p.scale));
 }
 
-template <bool F32, bool INTERLEAVED, bool VEC, bool SPLIT>
+template <bool F32, int BYTES, bool INTERLEAVED, bool SPLIT>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotParams p) {
-    using V = RotVec<F32, VEC>;
+    using V = RotVec<F32, BYTES>;
     // A unit is what a thread moves of every head: one vector of side-by-side pairs, two vectors half a rotated part apart (two single
     // values, in either layout), or one vector that is only copied.  The units cover a head, so a segment that is not turned (v) is
     // copied by the same units.
-    constexpr bool ONE = INTERLEAVED && VEC;
+    constexpr bool ONE = INTERLEAVED && V::N > 1;
     constexpr int RU = ONE ? V::N : 2 * V::N, PAIRS = RU / 2, ES = F32 ? 4 : 2;
     constexpr int BATCH = SPLIT ? 1 : ONE ? 4 : 2;  // heads: 64 bytes a batch
     extern __shared__ __align__(16) float2 s_cs[];  // [token of the block][pair]
@@ -211,11 +218,12 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_consta
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-template <bool F32>
-static int launch_rotary(RotParams p, bool interleaved, bool vec, cudaStream_t s) {
+template <bool F32, int BYTES>
+static int launch_rotary(RotParams p, bool interleaved, cudaStream_t s) {
     int rc, sms = 0, heads = 1;
     if ((rc = device_sm_count(&sms))) return rc;
-    const int n = vec ? (F32 ? 4 : 8) : 1, ru = interleaved && vec ? n : 2 * n;
+    constexpr int n = BYTES / (F32 ? 4 : 2);
+    const int ru = interleaved && n > 1 ? n : 2 * n;
     const int units = p.rot / ru + (p.d - p.rot) / n;
     p.lanes = units < ROT_THREADS ? units : ROT_THREADS;
     for (int g = 0; g < p.n_seg; ++g) heads = p.seg[g].heads > heads ? p.seg[g].heads : heads;
@@ -225,11 +233,12 @@ static int launch_rotary(RotParams p, bool interleaved, bool vec, cudaStream_t s
     while (p.split < heads && 2 * p.split * p.lanes <= ROT_THREADS && p.tokens * p.split * p.lanes < (int64_t)sms * 256) p.split *= 2;
     p.per_block = ROT_THREADS / (p.lanes * p.split);
     const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
-    void (*const kerns[2][2][2])(const RotParams) = {
-        {{rotary_kernel<F32, false, false, false>, rotary_kernel<F32, false, false, true>}, {rotary_kernel<F32, false, true, false>, rotary_kernel<F32, false, true, true>}},
-        {{rotary_kernel<F32, true, false, false>, rotary_kernel<F32, true, false, true>}, {rotary_kernel<F32, true, true, false>, rotary_kernel<F32, true, true, true>}}};
-    const auto kern = kerns[interleaved][vec][p.split > 1];
-    return check_cuda(launch_pdl(kern, dim3((unsigned)blocks), dim3(p.lanes * p.split * p.per_block), p.split > 1 ? (size_t)p.per_block * (p.rot / 2) * sizeof(float2) : 0, s, p), "rotary launch");
+    const bool split = p.split > 1;
+    void (*kern)(const RotParams) = interleaved ? (split ? rotary_kernel<F32, BYTES, true, true> : rotary_kernel<F32, BYTES, true, false>)
+                                                : (split ? rotary_kernel<F32, BYTES, false, true> : rotary_kernel<F32, BYTES, false, false>);
+    return check_cuda(launch_pdl(kern, dim3((unsigned)blocks), dim3(p.lanes * p.split * p.per_block),
+                                 split ? (size_t)p.per_block * (p.rot / 2) * sizeof(float2) : 0, s, p),
+                      "rotary launch");
 }
 
 }  // namespace quartet
@@ -249,17 +258,18 @@ extern "C" __attribute__((visibility("default"))) int quartet_rotary(int n_seg, 
     if (d < 2 || d > 65536 || rot < 2 || rot % 2 || rot > d || rot > 2 * ROT_MAX_PAIRS)
         return fail(QUARTET_E_SHAPE, "need an even rot, 2 <= rot <= min(d, %d) (got rot %lld, d %lld)", 2 * ROT_MAX_PAIRS, (long long)rot, (long long)d);
     const bool f32 = dtype == QUARTET_F32;
-    const int eb = f32 ? 4 : 2, per = 16 / eb;
+    const int eb = f32 ? 4 : 2;
     RotParams p{};
-    bool vec = d % per == 0 && (interleaved ? rot : rot / 2) % per == 0;
+    // every address that a thread forms is a sum of these: their common power of two is how much it may move at once
+    uint64_t bits = 16 | (uint64_t)d * eb | (uint64_t)(interleaved ? rot : rot / 2) * eb;
     for (int g = 0; g < n_seg; ++g) {
         const int64_t* st = strides6 + 6 * g;
         if (!src[g] || !dst[g]) return fail(QUARTET_E_NULL, "segment %d has a NULL pointer", g);
         if (heads[g] < 1 || heads[g] > 65536) return fail(QUARTET_E_SHAPE, "segment %d: need 1 <= heads <= 65536", g);
         if ((reinterpret_cast<uintptr_t>(src[g]) | reinterpret_cast<uintptr_t>(dst[g])) & (uintptr_t)(eb - 1))
             return fail(QUARTET_E_ALIGN, "segment %d is not aligned to its type", g);
-        vec = vec && aligned16(src[g]) && aligned16(dst[g]);
-        for (int k = 0; k < 6; ++k) vec = vec && st[k] % per == 0;
+        bits |= reinterpret_cast<uintptr_t>(src[g]) | reinterpret_cast<uintptr_t>(dst[g]);
+        for (int k = 0; k < 6; ++k) bits |= (uint64_t)st[k] * (uint64_t)eb;
         p.seg[g] = RotSeg{src[g], dst[g], st[0], st[1], st[2], st[3], st[4], st[5], heads[g], rotate[g] != 0};
     }
     if (reinterpret_cast<uintptr_t>(inv_freq) & 7u) return fail(QUARTET_E_ALIGN, "inv_freq must be 8-byte aligned");
@@ -272,5 +282,9 @@ extern "C" __attribute__((visibility("default"))) int quartet_rotary(int n_seg, 
     p.inv_freq = inv_freq, p.scale = scale, p.inverse = inverse != 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     p.tokens = batch * tokens;
-    return f32 ? launch_rotary<true>(p, interleaved != 0, vec, s) : launch_rotary<false>(p, interleaved != 0, vec, s);
+    const int bytes = (int)(bits & (~bits + 1));
+    const bool inter = interleaved != 0;
+    if (f32) return bytes == 16 ? launch_rotary<true, 16>(p, inter, s) : bytes == 8 ? launch_rotary<true, 8>(p, inter, s) : launch_rotary<true, 4>(p, inter, s);
+    if (bytes >= 8) return bytes == 16 ? launch_rotary<false, 16>(p, inter, s) : launch_rotary<false, 8>(p, inter, s);
+    return bytes == 4 ? launch_rotary<false, 4>(p, inter, s) : launch_rotary<false, 2>(p, inter, s);
 }

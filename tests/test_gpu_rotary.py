@@ -39,7 +39,7 @@ def check(got, want, m):
 
 
 @pytest.mark.parametrize("b,t,hq,hk,d,rot", [(1, 1, 1, 1, 2, 2), (2, 1, 32, 8, 128, 128), (1, 5, 3, 1, 96, 64), (3, 17, 5, 5, 128, 128), (2, 33, 4, 2, 80, 20),
-                                             (1, 130, 2, 1, 100, 50), (2, 7, 3, 3, 7, 6), (1, 3, 2, 2, 512, 512), (1, 4, 9, 3, 256, 64)])
+                                             (1, 130, 2, 1, 100, 50), (2, 7, 3, 3, 7, 6), (1, 3, 2, 2, 512, 512), (1, 4, 9, 3, 256, 64), (2, 40, 3, 2, 72, 72), (1, 50, 2, 2, 68, 36), (3, 9, 4, 1, 66, 66)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_apply_and_gradient(R, b, t, hq, hk, d, rot, dtype, interleaved):
