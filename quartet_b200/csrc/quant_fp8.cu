@@ -140,32 +140,80 @@ __global__ void __launch_bounds__(F8TileCfg<TRANS>::THREADS, F32 ? 2 : 4) quant_
 // 32 KB buffers, three CTAs on an SM).  One tile per CTA as above spends its time waiting: 59 us against 50 for both orientations of
 // 16384 x 4096 (45 against 33 for the transposed one alone, 0.94 of the memory's rate).  The transposed codes are put together in the tile's own buffer,
 // once every value of it is in registers.
-constexpr int DUAL_TILE = F8_TILE * F8_TILE * 2, DUAL_CTAS = 3;
-constexpr int DUAL_SMEM = 2 * DUAL_TILE + 8 * 64 * 4;
+//
+// Where the tensor starts on a 16-byte boundary and its rows do not (SHIFTED), the 16-byte units that hold a row's part are fetched, seventeen of
+// them, and the warps move the rows to their places in shared memory.  16384 x 4097: 74 us (66 in square blocks) against 96 with single
+// values loaded by threads; rows alone 55 us against 61 in the kernel above, so that those come here as well (TRANS off).  The extra pass is
+// bound by the integer pipe, and aligned rows do without it: 50 us against 62.
+constexpr int DUAL_CTAS = 3;
+template <bool SHIFTED>
+struct DualCfg {
+    static constexpr int PITCH = SHIFTED ? 272 : 256, TILE = F8_TILE * PITCH, SMEM = 2 * TILE + 8 * 64 * 4;
+};
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool inside) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(inside ? 16 : 0) : "memory");  // zeros outside
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");  // zeros behind the first `bytes`
 }
 
-template <bool E5M2, bool SQUARE, bool ROWS>
+// The 16-byte units that hold the tile's 128 rows x 256 bytes.  Nothing is read past the tensor's end; zeros behind it and below the last row.
+__device__ __forceinline__ void fetch_shifted(const Fp8QuantParams& p, uint8_t* buf, int64_t row0, int64_t col0, int tid) {
+    const int64_t end = p.rows * p.cols * 2;
+    auto unit = [&](int r, int u) {
+        const int64_t row = row0 + r, at = (((row * p.cols + col0) * 2) & ~(int64_t)15) + 16 * u;
+        const int64_t n = row < p.rows && at < end ? end - at : 0;
+        cp_async16(smem_u32(buf) + r * DualCfg<true>::PITCH + u * 16, p.x + (n ? at : 0), n < 16 ? (int)n : 16);
+    };
+#pragma unroll
+    for (int k = 0; k < 8; ++k) unit((tid >> 4) + 16 * k, tid & 15);
+    if (tid < F8_TILE) unit(tid, 16);
+}
+
+// Rows that were fetched from where their first unit starts move to where they start themselves, and values past the last column become zeros.
+// A warp does its sixteen rows four at a time, its lanes neighbouring words; a row's last word read is the last of its seventeen units.
+__device__ __forceinline__ void align_rows(const Fp8QuantParams& p, uint8_t* buf, int64_t row0, int64_t col0, int w, int lane) {
+    const uint32_t first = (uint32_t)(row0 + 16 * w) * (uint32_t)p.cols + (uint32_t)col0;   // only its low bits count
+    const int64_t n = p.cols - col0 - 2 * lane;   // values from this lane's first one to the row's end
+    const uint32_t m0 = n > 1 ? 0xFFFFFFFFu : n == 1 ? 0xFFFFu : 0u, m1 = n > 65 ? 0xFFFFFFFFu : n == 65 ? 0xFFFFu : 0u;
+#pragma unroll 1
+    for (int r = 0; r < 16; r += 4) {
+        uint32_t v[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t off = 2u * (first + (uint32_t)(r + u) * (uint32_t)p.cols) & 15u, bits = (off & 2u) * 8u;
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(buf + (16 * w + r + u) * DualCfg<true>::PITCH) + (off >> 2) + lane;
+            v[u][0] = __funnelshift_r(x[0], x[1], bits) & m0;
+            v[u][1] = __funnelshift_r(x[32], x[33], bits) & m1;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(buf + (16 * w + r + u) * DualCfg<true>::PITCH) + lane;
+            x[0] = v[u][0], x[32] = v[u][1];
+        }
+    }
+}
+
+template <bool E5M2, bool SQUARE, bool ROWS, bool TRANS, bool SHIFTED>
 __global__ void __launch_bounds__(F8_THREADS, DUAL_CTAS) quant_fp8_dual_kernel(const Fp8QuantParams p, const int tiles_x, const int64_t tiles) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t s_red[8];
-    constexpr int TOP = E5M2 ? 15 : 8;
+    constexpr int TOP = E5M2 ? 15 : 8, DUAL_PITCH = DualCfg<SHIFTED>::PITCH, DUAL_TILE = DualCfg<SHIFTED>::TILE;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + 2 * DUAL_TILE);  // [8 row groups][64 column pairs]
     const int tid = threadIdx.x, j = tid & 7, r0 = tid >> 3, w = tid >> 5, lane = tid & 31;
     const int64_t tiles_y = tiles / tiles_x;
 
     auto fetch = [&](uint8_t* buf, int64_t tile) {
         const int64_t ty = tile / tiles_x, row0 = ty * F8_TILE, col0 = (tile - ty * tiles_x) * F8_TILE;
-        if (p.vec) {
+        if constexpr (SHIFTED) {
+            fetch_shifted(p, buf, row0, col0, tid);
+        } else if (p.vec) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int64_t row = row0 + r0 + 32 * s, c = col0 + (j + 8 * i) * 8;
                     const bool in = row < p.rows && c < p.cols;
-                    cp_async16(buf + (r0 + 32 * s) * 256 + (j + 8 * i) * 16, p.x + (in ? row * p.cols + c : 0) * 2, in);
+                    cp_async16(smem_u32(buf) + (r0 + 32 * s) * DUAL_PITCH + (j + 8 * i) * 16, p.x + (in ? row * p.cols + c : 0) * 2, in ? 16 : 0);
                 }
         } else {
 #pragma unroll 1
@@ -173,7 +221,7 @@ __global__ void __launch_bounds__(F8_THREADS, DUAL_CTAS) quant_fp8_dual_kernel(c
                 RowPart<false> part;
                 part.load(p.x, p.rows, p.cols, 0, row0 + r0 + 32 * s, col0, j);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(buf + (r0 + 32 * s) * 256 + (j + 8 * i) * 16) = part.q[i];
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(buf + (r0 + 32 * s) * DUAL_PITCH + (j + 8 * i) * 16) = part.q[i];
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -194,12 +242,16 @@ __global__ void __launch_bounds__(F8_THREADS, DUAL_CTAS) quant_fp8_dual_kernel(c
         __syncthreads();
         const int64_t ty = tile / tiles_x, tx = tile - ty * tiles_x, row0 = ty * F8_TILE, col0 = tx * F8_TILE;
         uint32_t tile_byte = 0;
+        if constexpr (SHIFTED) {
+            align_rows(p, buf, row0, col0, w, lane);
+            __syncthreads();
+        }
         if constexpr (ROWS || SQUARE) {
             RowPart<false> part[4];
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) part[s].q[i] = *reinterpret_cast<const uint4*>(buf + (r0 + 32 * s) * 256 + (j + 8 * i) * 16);
+                for (int i = 0; i < 2; ++i) part[s].q[i] = *reinterpret_cast<const uint4*>(buf + (r0 + 32 * s) * DUAL_PITCH + (j + 8 * i) * 16);
             if constexpr (SQUARE) {
                 uint32_t m = 0u;
 #pragma unroll
@@ -228,59 +280,61 @@ __global__ void __launch_bounds__(F8_THREADS, DUAL_CTAS) quant_fp8_dual_kernel(c
                 }
             }
         }
-        // warp w: rows 16 w .. 16 w + 15 of column pairs lane and lane + 32
-        uint32_t raw[2][16];
+        if constexpr (TRANS) {
+            // warp w: rows 16 w .. 16 w + 15 of column pairs lane and lane + 32
+            uint32_t raw[2][16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) raw[h][i] = *reinterpret_cast<const uint32_t*>(buf + (16 * w + i) * 256 + (lane + 32 * h) * 4);
-            if (!SQUARE) {
-                Mag<false> m;
+                for (int i = 0; i < 16; ++i) raw[h][i] = *reinterpret_cast<const uint32_t*>(buf + (16 * w + i) * DUAL_PITCH + (lane + 32 * h) * 4);
+                if (!SQUARE) {
+                    Mag<false> m;
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) m.take(raw[h][i], raw[h][i + 1]);
-                s_max[w * 64 + lane + 32 * h] = m.packed();
-            }
-        }
-        __syncthreads();  // the buffer's values are in registers from here on
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int word = lane + 32 * h, col = 2 * word;
-            uint32_t sb0 = tile_byte, sb1 = tile_byte;
-            if (!SQUARE) {
-                uint32_t m = 0u;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) m = Mag<false>::join(m, s_max[k * 64 + word]);
-                sb0 = fp8_scale_byte(m << 16, TOP), sb1 = fp8_scale_byte(m & 0xFFFF0000u, TOP);
-            }
-            const f32x2_t inv = pack2(fp8_inv_scale(sb0), fp8_inv_scale(sb1));
-            uint32_t o0[4], o1[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float c0[4], c1[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const uint32_t x = raw[h][4 * k + t];
-                    unpack2(mul2(pack2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), inv), c0[t], c1[t]);
+                    for (int i = 0; i < 16; i += 2) m.take(raw[h][i], raw[h][i + 1]);
+                    s_max[w * 64 + lane + 32 * h] = m.packed();
                 }
-                o0[k] = cvt_fp8x4<E5M2>(c0[0], c0[1], c0[2], c0[3]);
-                o1[k] = cvt_fp8x4<E5M2>(c1[0], c1[1], c1[2], c1[3]);
             }
-            const int sw = (w ^ (word & 7)) << 4;  // eight neighbouring lanes write to eight different 16-byte units
-            *reinterpret_cast<uint4*>(buf + col * F8_TILE + sw) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-            *reinterpret_cast<uint4*>(buf + (col + 1) * F8_TILE + sw) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-            if (w == h) {
-                uint8_t* sf = p.sf_t + (tx * tiles_y + ty) * 512;
-                *reinterpret_cast<uint32_t*>(sf + (col & 31) * 16 + (col >> 5) * 4) = col0 + col < p.cols ? sb0 * 0x01010101u : 0u;
-                *reinterpret_cast<uint32_t*>(sf + ((col + 1) & 31) * 16 + (col >> 5) * 4) = col0 + col + 1 < p.cols ? sb1 * 0x01010101u : 0u;
-            }
-        }
-        __syncthreads();
+            __syncthreads();  // the buffer's values are in registers from here on
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int col = r0 + 32 * s;
-            if (col0 + col < p.cols)
-                *reinterpret_cast<uint4*>(p.codes_t + (col0 + col) * p.pitch_t + row0 + j * 16) =
-                    *reinterpret_cast<const uint4*>(buf + col * F8_TILE + ((j ^ ((col >> 1) & 7)) << 4));
+            for (int h = 0; h < 2; ++h) {
+                const int word = lane + 32 * h, col = 2 * word;
+                uint32_t sb0 = tile_byte, sb1 = tile_byte;
+                if (!SQUARE) {
+                    uint32_t m = 0u;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) m = Mag<false>::join(m, s_max[k * 64 + word]);
+                    sb0 = fp8_scale_byte(m << 16, TOP), sb1 = fp8_scale_byte(m & 0xFFFF0000u, TOP);
+                }
+                const f32x2_t inv = pack2(fp8_inv_scale(sb0), fp8_inv_scale(sb1));
+                uint32_t o0[4], o1[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float c0[4], c1[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t x = raw[h][4 * k + t];
+                        unpack2(mul2(pack2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)), inv), c0[t], c1[t]);
+                    }
+                    o0[k] = cvt_fp8x4<E5M2>(c0[0], c0[1], c0[2], c0[3]);
+                    o1[k] = cvt_fp8x4<E5M2>(c1[0], c1[1], c1[2], c1[3]);
+                }
+                const int sw = (w ^ (word & 7)) << 4;  // eight neighbouring lanes write to eight different 16-byte units
+                *reinterpret_cast<uint4*>(buf + col * F8_TILE + sw) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+                *reinterpret_cast<uint4*>(buf + (col + 1) * F8_TILE + sw) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+                if (w == h) {
+                    uint8_t* sf = p.sf_t + (tx * tiles_y + ty) * 512;
+                    *reinterpret_cast<uint32_t*>(sf + (col & 31) * 16 + (col >> 5) * 4) = col0 + col < p.cols ? sb0 * 0x01010101u : 0u;
+                    *reinterpret_cast<uint32_t*>(sf + ((col + 1) & 31) * 16 + (col >> 5) * 4) = col0 + col + 1 < p.cols ? sb1 * 0x01010101u : 0u;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int col = r0 + 32 * s;
+                if (col0 + col < p.cols)
+                    *reinterpret_cast<uint4*>(p.codes_t + (col0 + col) * p.pitch_t + row0 + j * 16) =
+                        *reinterpret_cast<const uint4*>(buf + col * F8_TILE + ((j ^ ((col >> 1) & 7)) << 4));
+            }
         }
         __syncthreads();  // the next trip fetches into this buffer
     }
@@ -326,22 +380,25 @@ static int launch_quant_fp8(const Fp8QuantParams& p, cudaStream_t s) {
     const dim3 grid((unsigned)((p.cols + 127) / 128), (unsigned)((p.rows + 127) / 128));
     return check_cuda(launch_pdl(kern, grid, dim3(F8TileCfg<TRANS>::THREADS), smem, s, p), "quant_fp8 launch");
 }
-template <bool E5M2, bool SQUARE, bool ROWS>
+template <bool E5M2, bool SQUARE, bool ROWS, bool TRANS, bool SHIFTED>
 static int launch_quant_dual(const Fp8QuantParams& p, cudaStream_t s) {
-    auto kern = quant_fp8_dual_kernel<E5M2, SQUARE, ROWS>;
+    auto kern = quant_fp8_dual_kernel<E5M2, SQUARE, ROWS, TRANS, SHIFTED>;
+    constexpr int smem = DualCfg<SHIFTED>::SMEM;
     static thread_local int smem_set = -1;
-    int rc = set_max_smem_once(kern, DUAL_SMEM, smem_set), sms = 0;
+    int rc = set_max_smem_once(kern, smem, smem_set), sms = 0;
     if (rc || (rc = device_sm_count(&sms))) return rc;
     const int tx = (int)((p.cols + 127) / 128);
     const int64_t tiles = tx * ((p.rows + 127) / 128);
     const unsigned grid = (unsigned)(tiles < (int64_t)sms * DUAL_CTAS ? tiles : (int64_t)sms * DUAL_CTAS);
-    return check_cuda(launch_pdl(kern, dim3(grid), dim3(F8_THREADS), DUAL_SMEM, s, p, tx, tiles), "quant_fp8 launch");
+    return check_cuda(launch_pdl(kern, dim3(grid), dim3(F8_THREADS), smem, s, p, tx, tiles), "quant_fp8 launch");
 }
 template <bool F32, bool E5M2, bool SQUARE>
 static int pick_quant_fp8(const Fp8QuantParams& p, cudaStream_t s) {
     if constexpr (!F32) {
-        if (p.codes_t) return p.codes ? launch_quant_dual<E5M2, SQUARE, true>(p, s) : launch_quant_dual<E5M2, SQUARE, false>(p, s);
-        return launch_quant_fp8<false, E5M2, SQUARE, true, false>(p, s);
+        const bool shifted = aligned16(p.x) && !p.vec;
+        if (!p.codes_t) return shifted ? launch_quant_dual<E5M2, SQUARE, true, false, true>(p, s) : launch_quant_fp8<false, E5M2, SQUARE, true, false>(p, s);
+        if (shifted) return p.codes ? launch_quant_dual<E5M2, SQUARE, true, true, true>(p, s) : launch_quant_dual<E5M2, SQUARE, false, true, true>(p, s);
+        return p.codes ? launch_quant_dual<E5M2, SQUARE, true, true, false>(p, s) : launch_quant_dual<E5M2, SQUARE, false, true, false>(p, s);
     } else if (p.codes && p.codes_t) {
         return launch_quant_fp8<true, E5M2, SQUARE, true, true>(p, s);
     } else {

@@ -54,6 +54,30 @@ def test_quantizer_equals_the_definition(ops, rows, cols, dtype, square, fmt):
     assert torch.equal(only[2].view(torch.uint8), got[2].view(torch.uint8)) and torch.equal(only[3], got[3]) and only[0] is None
 
 
+@pytest.mark.parametrize("rows,cols", [(2600, 2903), (2600, 2902), (2611, 2900), (300, 121), (1, 9)])
+@pytest.mark.parametrize("offset", [0, 1, 2, 8])
+@pytest.mark.parametrize("square", [False, True])
+def test_quantizer_reads_rows_wherever_they_start(ops, rows, cols, offset, square):
+    """Rows that start on any even byte, between values that are not numbers, in more tiles than CTAs: as from a padded copy with aligned rows."""
+    flat = torch.full((rows * cols + 64,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    x = flat[offset:offset + rows * cols].view(rows, cols)
+    x.copy_(_x(rows, cols, torch.bfloat16, rows + cols))
+    padded = torch.zeros(rows, -(-cols // 128) * 128, dtype=torch.bfloat16, device="cuda")
+    padded[:, :cols] = x
+    want, got = (ops.quant_fp8(t, E4M3, square=square, transpose=True) for t in (padded, x))
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+    assert torch.equal(got[2].view(torch.uint8), want[2][:cols].view(torch.uint8))
+    # [column blocks, row blocks, 32, 4, 4]: the bytes of columns past the last one are zeros, where the padded copy has those of columns of zeros
+    blocks = want[3].view(-1, -(-rows // 128), 32, 4, 4).clone()
+    if cols % 128:
+        blocks[-1] *= (torch.arange(128).view(4, 32).T < cols % 128).cuda()[None, :, :, None]
+    assert torch.equal(got[3].view_as(blocks), blocks)
+    only = ops.quant_fp8(x, E4M3, square=square)
+    assert torch.equal(only[0].view(torch.uint8), got[0].view(torch.uint8)) and torch.equal(only[1], got[1])
+    only = ops.quant_fp8(x, E4M3, square=square, rows=False, transpose=True)
+    assert torch.equal(only[2].view(torch.uint8), got[2].view(torch.uint8)) and torch.equal(only[3], got[3])
+
+
 def test_quantizer_rounds_every_code_boundary_to_even(ops):
     """Every value of the formats and every midpoint between two, in a block whose scale is 1."""
     for fmt, top in ((E4M3, 448.0), (E5M2, 57344.0)):
