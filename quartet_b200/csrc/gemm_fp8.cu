@@ -294,6 +294,9 @@ static int launch_split(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8
 
 // ---------------------------------------------------------------------------
 // CTA pairs (cta_group::2): 256 x 256 results a pair, persistent
+//
+// Narrower tiles would fill the last wave better where N is a small multiple of 64 or 32, but a product of 160 columns takes 0.83 of the time of one
+// of 256: 8192 x 8192 x 4096 in 198 us, 227 with 192 columns, 263 with 160; 4096 x 640 x 32000 in 86, 89 and 92.
 // ---------------------------------------------------------------------------
 struct PairCfg {
     static constexpr int BN = 256;
