@@ -152,6 +152,15 @@ def test_product_within_its_bound(ops, mnk):
     _product(ops, *mnk, out_dtype=torch.bfloat16, alpha=0.375)
 
 
+@pytest.mark.parametrize("mnk", [(130, 4010, 8192), (257, 1999, 8192),                      # 256 rows of A in a CTA, one and two blocks of them
+                                 (300, 11003, 640), (66, 19000, 256),                       # more tiles than SMs, two to an SM
+                                 (100, 640, 4096), (140, 1200, 2000), (129, 4096, 1000),    # clusters of eight, four and two
+                                 (2300, 4101, 256), (2300, 4100, 140), (60000, 100, 128), (40001, 203, 100), (38000, 64, 128)])  # pairs
+def test_product_in_every_form(ops, mnk):
+    _product(ops, *mnk)
+    _product(ops, *mnk, out_dtype=torch.bfloat16)
+
+
 @pytest.mark.parametrize("fa,fb", [(E5M2, E4M3), (E4M3, E5M2), (E5M2, E5M2)])
 def test_product_of_mixed_formats(ops, fa, fb):
     _product(ops, 200, 320, 900, fa, fb)
@@ -212,6 +221,23 @@ def test_product_leaves_memory_beside_its_result_alone(ops):
                                                  ops._stream())
             assert rc == 0
             assert torch.equal(buf[:M, :N], want) and bool((buf[M:] == 7).all()) and bool((buf[:, N:] == 7).all())
+
+
+def test_large_products_leave_memory_beside_their_result_alone(ops):
+    """As above, where pairs of CTAs store whole 16-byte units and the rest value by value, and where rows are split between CTAs."""
+    from quartet_b200 import _lib
+
+    for M, N, K in ((2300, 4101, 128), (2300, 4100, 128), (40001, 199, 128), (40001, 65, 128), (300, 11003, 256), (130, 4010, 8192)):
+        for dt, code in ((torch.bfloat16, 0), (torch.float32, 1)):
+            a, b = torch.randn(M, K, device="cuda"), torch.randn(N, K, device="cuda")
+            (ac, asf, _, _), (bc, bsf, _, _) = ops.quant_fp8(a), ops.quant_fp8(b, square=True)
+            want = ops.gemm_fp8_tn(ac, asf, bc, bsf, out_dtype=dt)
+            buf = torch.full((M + 130, (N + 15) // 8 * 8), 7.0, dtype=dt, device="cuda")
+            rc = _lib.load().quartet_gemm_fp8_tn(ops._ptr(ac), ops._ptr(asf), 0, ops._ptr(bc), ops._ptr(bsf), 0, M, N, K, 1.0, ops._ptr(buf), code, buf.shape[1],
+                                                 ops._stream())
+            assert rc == 0
+            assert torch.equal(buf[:M, :N], want) and bool((buf[M:] == 7).all()) and bool((buf[:, N:] == 7).all())
+    assert ops.device_status() == 0
 
 
 def test_products_repeat_bit_for_bit(ops):
