@@ -17,15 +17,20 @@ from .. import ops, torch_ops  # noqa: F401  (torch_ops registers the operators 
 from .producers import _out_dtype
 
 
+def _forward(x, w, need_dx, need_dw, out_dtype):
+    x2 = x if x.dim() == 2 else x.reshape(-1, w.shape[1])
+    y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0]), saved
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, grad_dtype, out_dtype):
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        x2 = x if x.dim() == 2 else x.reshape(-1, w.shape[1])
-        y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
+        y, saved = _forward(x, w, need_dx, need_dw, out_dtype)
         ctx.save_for_backward(saved)
         ctx.x_shape, ctx.args, ctx.kept = x.shape, (w.shape[1], grad_dtype, x.dtype, w.dtype), (need_dx, need_dw)
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+        return y
 
     @staticmethod
     def backward(ctx, e):
@@ -57,7 +62,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, grad_dtype: torch.dtype
     if torch.compiler.is_compiling():
         need = torch.is_grad_enabled()
         return torch.ops.quartet_b200.fp8_linear_fwd(x, weight, grad_dtype, out_dtype, need and x.requires_grad, need and weight.requires_grad)[0]
-    return _Fp8LinearFn.apply(x, weight, grad_dtype, out_dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _Fp8LinearFn.apply(x, weight, grad_dtype, out_dtype)
+    return _forward(x, weight, False, False, out_dtype)[0]  # nothing is kept, so neither transpose is made
 
 
 class Fp8Linear(nn.Linear):

@@ -334,6 +334,23 @@ def test_layer_shapes_strides_streams_and_empty_batches(ops):
     assert list(lin.state_dict()) == ["weight", "bias"]
 
 
+def test_layer_without_gradients_keeps_nothing(ops, monkeypatch):
+    from quartet_b200.quantization import Fp8Linear
+
+    seen, real = [], ops.fp8_linear_fwd
+    monkeypatch.setattr(ops, "fp8_linear_fwd", lambda x, w, need_dx, need_dw, dt: seen.append((need_dx, need_dw)) or real(x, w, need_dx, need_dw, dt))
+    lin, x = Fp8Linear(200, 96, device="cuda"), torch.randn(3, 5, 200, device="cuda")
+    want = lin(x)
+    assert want.requires_grad and seen == [(False, True)]
+    with torch.no_grad():
+        got = lin(x)
+    with torch.inference_mode():
+        inf = lin(x)
+    lin.requires_grad_(False)
+    assert torch.equal(got, want) and torch.equal(inf, want) and torch.equal(lin(x), want) and not got.requires_grad
+    assert seen[1:] == [(False, False)] * 3
+
+
 def test_layer_captured_and_replayed(ops):
     """Forward and backward in one graph, replayed on new inputs; a second graph beside it does not disturb it."""
     from quartet_b200.quantization import fp8_linear
