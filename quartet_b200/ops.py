@@ -723,6 +723,7 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None, total=None):
     with _on(dev):
         rc = _lib.load().quartet_clip_grads(len(tensors), _at(ptrs), _at(optrs), _at(numels), _at(dts), _at(odts), kind, float(max_norm), _ptr(total), _ptr(work), _ptr(norm), _stream())
     _lib.check(rc, "quartet_clip_grads")
+    torch.autograd.graph.increment_version(tensors if out is None else out)  # a graph that saved one of them then refuses to use it
     return norm
 
 

@@ -165,3 +165,18 @@ def test_refusals(ops):
         with pytest.raises(ValueError):
             call()
     assert ops.grad_norm([x, x]).item() > 0   # the same tensor twice counts twice in a norm; clipped twice it is refused
+
+
+def test_clipping_is_seen_by_a_graph_that_saved_a_gradient(ops):
+    """As after any change in place: the backward of a graph that saved the gradient raises, and does not use the scaled values."""
+    w = torch.full((300,), 3.0, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((w * w).sum(), w, create_graph=True)
+    kept = g.detach()
+    loss = (kept * w).sum()
+    ops.clip_grads([kept], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    out, kept = torch.empty(300, device="cuda"), torch.ones(300, device="cuda")
+    version, before = out._version, kept._version
+    ops.clip_grads([kept], 1.0, out=[out])
+    assert out._version > version and kept._version == before
