@@ -17,6 +17,8 @@
 
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 namespace quartet {
 
 // Instruction descriptor, kind::mxf8f6f4, UE8M0 scales, both operands K-major.
@@ -402,9 +404,48 @@ __device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const ui
     }
 }
 
+// One product, or two that do not depend on one another: the second one's tiles fill the pairs that the first one's last round leaves idle.
+struct PairMaps {
+    CUtensorMap a, b, d, sfb;
+};
+struct PairSecond {
+    PairMaps tm;
+    Fp8GemmParams g;
+    int extra;  // how many of its tiles take as long as one of the first product's
+};
+__device__ __forceinline__ int pair_rows(const Fp8GemmParams& p) { return (int)((p.M + 255) / 256); }
+__device__ __forceinline__ int pair_cols(const Fp8GemmParams& p) { return (int)((p.N + 255) / 256); }
+
+// The tiles of a pair of CTAs.  The first product's are dealt out in rounds; of the second one's, the pairs that the last of these rounds left out
+// take `extra` each, and all take the rest in rounds that begin with them.
+template <bool TWO>
+struct PairTiles {
+    int n, tiles0, tiles1, first1, step1, end1, first2, at, stage = 0;
+    __device__ __forceinline__ PairTiles(int t0, int t1, int extra, int pair, int n_pairs) : n(n_pairs), tiles0(t0), tiles1(t1), at(pair) {
+        if (!TWO) return;
+        const int busy = tiles0 % n;                 // pairs that the last round takes; 0: all
+        step1 = n - busy;
+        end1 = busy ? min(tiles1, step1 * extra) : 0;
+        first1 = pair >= busy ? pair - busy : end1;
+        first2 = end1 + (pair >= busy ? pair - busy : pair + step1);
+    }
+    __device__ __forceinline__ bool next(int& product, int& tile) {
+        if (!TWO) {
+            product = 0, tile = at, at += n;
+            return tile < tiles0;
+        }
+        if (stage == 0 && at >= tiles0) stage = 1, at = first1;
+        if (stage == 1 && at >= end1) stage = 2, at = first2;
+        product = stage > 0, tile = at;
+        at += stage == 1 ? step1 : n;
+        return stage < 2 || tile < tiles1;
+    }
+};
+
+template <bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_d,
-                         const __grid_constant__ CUtensorMap tm_sfb, const Fp8GemmParams p) {
+                         const __grid_constant__ CUtensorMap tm_sfb, const Fp8GemmParams p0, const __grid_constant__ PairSecond p1) {
     using C = PairCfg;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
@@ -461,20 +502,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     pdl_launch_dependents();
     pdl_wait();
 
-    const int m_pairs = (int)((p.M + 255) / 256), n_tiles = (int)((p.N + 255) / 256);
-    const int m_blocks = (int)((p.M + 127) / 128);
-    const int n_tiles_total = m_pairs * n_tiles;
-    const int n_clusters = gridDim.x >> 1, cluster_id = blockIdx.x >> 1;
-    const int k_stages = p.k_chunks;
+    const int m_pairs0 = pair_rows(p0), n_tiles0 = pair_cols(p0), k_stages0 = p0.k_chunks;
+    PairTiles<TWO> tiles(m_pairs0 * n_tiles0, TWO ? pair_rows(p1.g) * pair_cols(p1.g) : 0, TWO ? p1.extra : 0, blockIdx.x >> 1, gridDim.x >> 1);
+    int product, tile, m_pair, n_blk;
+    auto second = [&]() { return TWO && product; };
+    auto coords = [&]() { tile_coords(tile, second() ? pair_rows(p1.g) : m_pairs0, second() ? pair_cols(p1.g) : n_tiles0, m_pair, n_blk); };
 
     if (warp == 0 || warp == 10 || warp == 15) {
         if (lane == 0) {
             const int role = warp == 0 ? 0 : (warp == 10 ? 1 : 2);
             const uint64_t keep = l2_policy_evict_last();
             uint32_t s = 0, ph = 0;
-            for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
-                int m_pair, n_blk;
-                tile_coords(tile, m_pairs, n_tiles, m_pair, n_blk);
+            while (!*dead && tiles.next(product, tile)) {
+                const Fp8GemmParams& p = second() ? p1.g : p0;
+                const int k_stages = second() ? p1.g.k_chunks : k_stages0;
+                coords();
+                const int m_blocks = (int)((p.M + 127) / 128);
                 const int m_blk = m_pair * 2 + (int)rank;
                 const int n0 = n_blk * C::BN;
                 // a second row block past the last one reads zero rows; its scales are the last block's, there being none of its own
@@ -483,14 +526,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     if (!gemm_wait(role == 2 ? &sf_free[s] : &empty[s], ph ^ 1, WAIT_GEMM_EMPTY, dead)) break;
                     if (role == 0) {
                         mbar_arrive_expect_tx(&full[s], C::A_BYTES);
-                        tma_load_2d_hint(s_a + s * C::A_BYTES, &tm_a, ks * 128, m_blk * 128, &full[s], keep);
+                        tma_load_2d_hint(s_a + s * C::A_BYTES, second() ? &p1.tm.a : &tm_a, ks * 128, m_blk * 128, &full[s], keep);
                     } else if (role == 1) {
                         mbar_arrive_expect_tx(&full[s], C::B_BYTES);
-                        tma_load_2d_hint(s_b + s * C::B_BYTES, &tm_b, ks * 128, n0 + (int)rank * 128, &full[s], keep);
+                        tma_load_2d_hint(s_b + s * C::B_BYTES, second() ? &p1.tm.b : &tm_b, ks * 128, n0 + (int)rank * 128, &full[s], keep);
                     } else {
                         mbar_arrive_expect_tx(&sf_land[s], C::SFA_BYTES + C::SFB_BYTES);
                         bulk_load_hint(s_sfa + s * C::SFA_BYTES, sfa_src + (int64_t)ks * 512, C::SFA_BYTES, &sf_land[s], keep);
-                        tma_load_2d_hint(s_sfb + s * C::SFB_BYTES, &tm_sfb, ks * 128, n0 / 128, &sf_land[s], keep);
+                        tma_load_2d_hint(s_sfb + s * C::SFB_BYTES, second() ? &p1.tm.sfb : &tm_sfb, ks * 128, n0 / 128, &sf_land[s], keep);
                     }
                     if (++s == C::STAGES) s = 0, ph ^= 1;
                 }
@@ -499,11 +542,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else if (warp == 1) {
         if (leader) {
             uint32_t s = 0, ph = 0, slot = 0, aph = 0, acc_it = 0;
-            const uint32_t id0 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 0), id1 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 1);
-            const uint32_t id2 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 2), id3 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 3);
             const uint32_t a_base = smem_u32(s_a), b_base = smem_u32(s_b);
             const uint32_t empty_own = smem_u32(&empty[0]), accf_own = smem_u32(acc_full);
-            for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
+            while (!*dead && tiles.next(product, tile)) {
+                const Fp8GemmParams& p = second() ? p1.g : p0;
+                const int k_stages = second() ? p1.g.k_chunks : k_stages0;
+                const uint32_t id0 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 0), id1 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 1);
+                const uint32_t id2 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 2), id3 = make_idesc_fp8(256, C::BN, p.a_e5m2, p.b_e5m2, 3);
                 if (!gemm_wait(acc_empty, aph ^ 1, WAIT_GEMM_ACC_EMPTY, dead)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (acc_it & 1) * C::ACC_SHIFT;
@@ -532,7 +577,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else if (warp >= 6 && warp <= 9) {
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         uint32_t it = 0;
-        for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters) {
+        while (!*dead && tiles.next(product, tile)) {
+            const int k_stages = second() ? p1.g.k_chunks : k_stages0;
             for (int ks = 0; ks < k_stages; ++ks, ++it) {
                 const int s = it % C::STAGES;
                 const uint32_t ph = (it / C::STAGES) & 1;
@@ -563,9 +609,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const int q = warp & 3, par = warp >= 11 ? 1 : 0;
         uint8_t* stg = s_stg + (par * 4 + q) * (C::NBUF * 4096);
         uint32_t acc_it = 0, n_stores = 0;
-        for (int tile = cluster_id; tile < n_tiles_total && !*dead; tile += n_clusters, ++acc_it) {
-            int m_pair, n_blk;
-            tile_coords(tile, m_pairs, n_tiles, m_pair, n_blk);
+        for (; !*dead && tiles.next(product, tile); ++acc_it) {
+            const Fp8GemmParams& p = second() ? p1.g : p0;
+            const CUtensorMap* d_map = second() ? &p1.tm.d : &tm_d;
+            coords();
             const int n0 = n_blk * C::BN;
             const int row0 = (m_pair * 2 + (int)rank) * 128 + q * 32;
             if (!gemm_wait(acc_full, acc_it & 1, WAIT_GEMM_ACC_FULL, dead)) break;
@@ -581,11 +628,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty), 0));
             const bool rows = row0 < p.M;
-            if (rows && n0 + c0 < p.N) store_block64<C::NBUF>(r0, r1, p, &tm_d, row0, n0 + c0, stg, n_stores, lane);
+            if (rows && n0 + c0 < p.N) store_block64<C::NBUF>(r0, r1, p, d_map, row0, n0 + c0, stg, n_stores, lane);
             tc_ld32(t0 + c1, r0);
             tc_ld32(t0 + c1 + 32, r1);
             tc_wait_ld();
-            if (rows && n0 + c1 < p.N) store_block64<C::NBUF>(r0, r1, p, &tm_d, row0, n0 + c1, stg, n_stores, lane);
+            if (rows && n0 + c1 < p.N) store_block64<C::NBUF>(r0, r1, p, d_map, row0, n0 + c1, stg, n_stores, lane);
             tc_fence_before();  // all of this tile's tensor-memory reads are complete before the warp's next arrive
         }
         if (lane == 0) bulk_wait0();
@@ -603,22 +650,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     }
 }
 
-static int launch_pair(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t stream) {
-    using C = PairCfg;
-    CUtensorMap tm_a, tm_b, tm_d, tm_sfb;
-    int rc = make_tmap_2d(&tm_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.M, K, 128, 128, 3);
+static int pair_maps(PairMaps* m, const Fp8Product& x) {
+    const Fp8GemmParams& p = x.g;
+    const int64_t K = (int64_t)p.k_chunks * 128;
+    int rc = make_tmap_2d(&m->a, x.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.M, K, 128, 128, 3);
     if (rc) return rc;
-    if ((rc = make_tmap_2d(&tm_b, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.N, K, 128, 128, 3))) return rc;
+    if ((rc = make_tmap_2d(&m->b, x.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, p.N, K, 128, 128, 3))) return rc;
     if (p.d_f32)
-        rc = make_tmap_2d(&tm_d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.N & ~(int64_t)3, p.M, (uint64_t)p.ldd * 4, 32, 32, 3);
+        rc = make_tmap_2d(&m->d, p.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.N & ~(int64_t)3, p.M, (uint64_t)p.ldd * 4, 32, 32, 3);
     else
-        rc = make_tmap_2d(&tm_d, p.d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.N & ~(int64_t)7, p.M, (uint64_t)p.ldd * 2, 64, 32, 3);
+        rc = make_tmap_2d(&m->d, p.d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.N & ~(int64_t)7, p.M, (uint64_t)p.ldd * 2, 64, 32, 3);
     if (rc) return rc;
     // B's scales as 32-bit words: a row for each 128-row block, 128 words a chunk; a stage takes one chunk of two row blocks
-    if ((rc = make_tmap_2d(&tm_sfb, p.b_sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (uint64_t)p.k_chunks * 128, (uint64_t)((p.N + 127) / 128),
-                           (uint64_t)p.k_chunks * 512, 128, 2, 0)))
-        return rc;
-    auto kern = gemm_fp8_pair_kernel;
+    return make_tmap_2d(&m->sfb, p.b_sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (uint64_t)p.k_chunks * 128, (uint64_t)((p.N + 127) / 128), (uint64_t)p.k_chunks * 512, 128,
+                        2, 0);
+}
+
+// One product, or two of which the first has the longer contraction.
+template <bool TWO>
+static int launch_pair(const Fp8Product* x, cudaStream_t stream) {
+    using C = PairCfg;
+    PairMaps first;
+    PairSecond second{};
+    int64_t tiles = 0;
+    int rc = pair_maps(&first, x[0]);
+    if (rc || (TWO && (rc = pair_maps(&second.tm, x[1])))) return rc;
+    for (int i = 0; i < (TWO ? 2 : 1); ++i) tiles += ((x[i].g.M + 255) / 256) * ((x[i].g.N + 255) / 256);
+    if (TWO) second.g = x[1].g, second.extra = x[0].g.k_chunks / x[1].g.k_chunks;
+    auto kern = gemm_fp8_pair_kernel<TWO>;
     static thread_local int smem_set = -1;
     if ((rc = set_max_smem_once(kern, C::SMEM, smem_set))) return rc;
     int dev = 0, sms = 0;
@@ -638,9 +697,8 @@ static int launch_pair(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8G
         if (n < 1) return fail(QUARTET_E_CUDA, "no CTA pair can be resident");
         cached_dev = dev, cached_clusters = n;
     }
-    const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
     const int clusters = (int)(tiles < cached_clusters ? tiles : cached_clusters);
-    return check_cuda(launch_pdl(kern, dim3(clusters * 2), dim3(PAIR_THREADS), C::SMEM, stream, tm_a, tm_b, tm_d, tm_sfb, p), "gemm_fp8 launch");
+    return check_cuda(launch_pdl(kern, dim3(clusters * 2), dim3(PAIR_THREADS), C::SMEM, stream, first.a, first.b, first.d, first.sfb, x[0].g, second), "gemm_fp8 launch");
 }
 
 QUARTET_DEFINE_STATUS_READER(status_gemm_fp8)
@@ -684,22 +742,23 @@ static int resident_clusters(const int (**out)[4]) {
 constexpr struct { int chunk, start, again; } COST_PAIR{6, 115, 35};
 constexpr struct { int chunk, start, join; } COST_256{6, 140, 30}, COST_128{5, 105, 30}, COST_128_TWO{5, 150, 30}, COST_FEW{5, 150, 8};
 
-static int product(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmParams& p, cudaStream_t s) {
-    if (gemv_fits(p.M, K)) return gemv_fp8_codes(a, b, p, s);
+enum class Way { FEW_TOKENS, PAIR, ROWS_256, ROWS_128, ROWS_128_TWO, ROWS_FEW };
+
+static int pick_way(const Fp8GemmParams& p, Way* way, int* splits, int64_t* cost) {
+    *way = Way::FEW_TOKENS, *splits = 1, *cost = 0;
+    if (gemv_fits(p.M, (int64_t)p.k_chunks * 128)) return QUARTET_OK;
     const int (*resident)[4] = nullptr;
     int rc = resident_clusters(&resident);
     if (rc) return rc;
     auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    enum { PAIR, ROWS_256, ROWS_128, ROWS_128_TWO, ROWS_FEW } way = PAIR;
-    int splits = 1;
-    int64_t least = INT64_MAX;
-    auto consider = [&](decltype(way) w, int sp, int64_t cost) {
-        if (cost < least) least = cost, way = w, splits = sp;
+    *cost = INT64_MAX;
+    auto consider = [&](Way w, int sp, int64_t c) {
+        if (c < *cost) *cost = c, *way = w, *splits = sp;
     };
     const int64_t n_tiles = ceil_div(p.N, 128);
     if (p.M > 64 && p.N >= 64) {
         const int64_t rounds = ceil_div(ceil_div(p.M, 256) * ceil_div(p.N, 256), (*resident)[1]);
-        consider(PAIR, 1, rounds * COST_PAIR.chunk * p.k_chunks + COST_PAIR.start + (rounds - 1) * COST_PAIR.again);
+        consider(Way::PAIR, 1, rounds * COST_PAIR.chunk * p.k_chunks + COST_PAIR.start + (rounds - 1) * COST_PAIR.again);
     }
     for (int i = 0; i < 4 && (1 << i) <= p.k_chunks && (*resident)[i] > 0; ++i) {
         const int sp = 1 << i;
@@ -707,23 +766,63 @@ static int product(const uint8_t* a, const uint8_t* b, int64_t K, const Fp8GemmP
         auto start = [&](const auto& c) { return c.start + (sp > 1 ? c.join : 0); };
         if (p.M > 64) {
             const int64_t rounds = ceil_div(n_tiles * ceil_div(p.M, 128), slots), rounds_256 = ceil_div(n_tiles * ceil_div(p.M, 256), slots);
-            if (p.M > 128 && sp < 8) consider(ROWS_256, sp, rounds_256 * (COST_256.chunk * chunks + start(COST_256)));
-            consider(ROWS_128, sp, rounds * (COST_128.chunk * chunks + start(COST_128)));
+            if (p.M > 128 && sp < 8) consider(Way::ROWS_256, sp, rounds_256 * (COST_256.chunk * chunks + start(COST_256)));
+            consider(Way::ROWS_128, sp, rounds * (COST_128.chunk * chunks + start(COST_128)));
             // two CTAs on an SM share its tensor core, but the beginning and end of one run under the other's products
-            consider(ROWS_128_TWO, sp, rounds * COST_128_TWO.chunk * chunks + (rounds + 1) / 2 * start(COST_128_TWO));
+            consider(Way::ROWS_128_TWO, sp, rounds * COST_128_TWO.chunk * chunks + (rounds + 1) / 2 * start(COST_128_TWO));
         } else {
             // with few rows the second one costs three quarters of a round: they wait for memory more than for the tensor core
             const int64_t rounds = ceil_div(n_tiles * ceil_div(p.M, p.M > 32 ? 64 : 32), slots);
-            consider(ROWS_FEW, sp, (rounds / 2 * 7 + rounds % 2 * 4) * COST_FEW.chunk * chunks / 4 + (rounds + 1) / 2 * start(COST_FEW));
+            consider(Way::ROWS_FEW, sp, (rounds / 2 * 7 + rounds % 2 * 4) * COST_FEW.chunk * chunks / 4 + (rounds + 1) / 2 * start(COST_FEW));
         }
     }
+    return QUARTET_OK;
+}
+
+static int run_way(const Fp8Product& x, Way way, int splits, cudaStream_t s) {
+    const int64_t K = (int64_t)x.g.k_chunks * 128;
     switch (way) {
-        case PAIR: return launch_pair(a, b, K, p, s);
-        case ROWS_256: return launch_split<256, 1>(a, b, K, p, splits, s);
-        case ROWS_128: return launch_split<128, 1>(a, b, K, p, splits, s);
-        case ROWS_128_TWO: return launch_split<128, 2>(a, b, K, p, splits, s);
-        default: return p.M > 32 ? launch_split<64, 2>(a, b, K, p, splits, s) : launch_split<32, 2>(a, b, K, p, splits, s);
+        case Way::FEW_TOKENS: return gemv_fp8_codes(x.a, x.b, x.g, s);
+        case Way::PAIR: return launch_pair<false>(&x, s);
+        case Way::ROWS_256: return launch_split<256, 1>(x.a, x.b, K, x.g, splits, s);
+        case Way::ROWS_128: return launch_split<128, 1>(x.a, x.b, K, x.g, splits, s);
+        case Way::ROWS_128_TWO: return launch_split<128, 2>(x.a, x.b, K, x.g, splits, s);
+        default: return x.g.M > 32 ? launch_split<64, 2>(x.a, x.b, K, x.g, splits, s) : launch_split<32, 2>(x.a, x.b, K, x.g, splits, s);
     }
+}
+
+static int product(const Fp8Product& x, cudaStream_t s) {
+    Way way;
+    int64_t cost;
+    int splits = 1, rc = pick_way(x.g, &way, &splits, &cost);
+    return rc ? rc : run_way(x, way, splits, s);
+}
+
+// Two products that do not depend on one another: in one launch of CTA pairs where by the model that takes 11/12 of the two at most, as the second one
+// then fills what the first one's last round leaves idle.  us of a whole backward pass, two launches / one: 4096 x 32000, K 640 263 / 249; 8192 x 5120,
+// K 1024 112-145 / 95-117; 1000 x 3000, K 2000 31-42 / 23-32; 300 x 2600, K 2600 23-31 / 23-25.  Where it would save 5 % of the chunks (8187 x 11008,
+// K 4096) the busier chip runs slower by as much, 578 / 582.
+int product_two(const Fp8Product& x, const Fp8Product& y, cudaStream_t s) {
+    Way wx, wy;
+    int64_t cost_x, cost_y;
+    int sx = 1, sy = 1, rc = pick_way(x.g, &wx, &sx, &cost_x);
+    if (rc || (rc = pick_way(y.g, &wy, &sy, &cost_y))) return rc;
+    auto for_pairs = [](const Fp8GemmParams& g) { return g.M > 64 && g.N >= 64; };
+    if (wx != Way::FEW_TOKENS && wy != Way::FEW_TOKENS && for_pairs(x.g) && for_pairs(y.g)) {
+        const int (*resident)[4] = nullptr;
+        if ((rc = resident_clusters(&resident))) return rc;
+        const int64_t n = (*resident)[1], cx = x.g.k_chunks, cy = y.g.k_chunks;
+        auto tiles = [](const Fp8GemmParams& g) { return ((g.M + 255) / 256) * ((g.N + 255) / 256); };
+        const int64_t tx = tiles(x.g), ty = tiles(y.g), rounds = (tx + ty + n - 1) / n;
+        const int64_t chunks = std::max((tx * cx + ty * cy + n - 1) / n, std::max(cx, cy));
+        const int64_t joined = COST_PAIR.chunk * chunks + COST_PAIR.start + (rounds - 1) * COST_PAIR.again;
+        if (12 * joined <= 11 * (cost_x + cost_y)) {
+            const Fp8Product both[2] = {cx >= cy ? x : y, cx >= cy ? y : x};
+            return launch_pair<true>(both, s);
+        }
+    }
+    rc = run_way(x, wx, sx, s);
+    return rc ? rc : run_way(y, wy, sy, s);
 }
 
 }  // namespace quartet
@@ -750,7 +849,7 @@ extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_tn(const 
     p.k_chunks = (int)(K / 128);
     p.a_e5m2 = a_fmt, p.b_e5m2 = b_fmt;
     p.alpha = alpha, p.d = d, p.d_f32 = d_dtype == QUARTET_F32;
-    return product(a, b, K, p, static_cast<cudaStream_t>(stream));
+    return product(Fp8Product{a, b, p}, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" __attribute__((visibility("default"))) int64_t quartet_linear_fp8_workspace_bytes(int64_t M, int64_t K) {

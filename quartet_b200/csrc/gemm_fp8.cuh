@@ -16,6 +16,13 @@ struct Fp8GemmParams {
     int d_f32;
 };
 
+// A product and its operands' codes.
+struct Fp8Product {
+    const uint8_t *a, *b;
+    Fp8GemmParams g;
+};
+int product_two(const Fp8Product& x, const Fp8Product& y, cudaStream_t s);
+
 // Up to eight rows (gemv_fp8.cu): from codes, or from values that the kernel quantizes.  gemv_fits: whether its shared memory holds them.
 bool gemv_fits(int64_t M, int64_t K);
 int gemv_fp8_codes(const uint8_t* a, const uint8_t* b, const Fp8GemmParams& g, cudaStream_t s);

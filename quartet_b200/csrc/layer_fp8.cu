@@ -2,8 +2,9 @@
 // order.  A caller in Python pays some 50 us for the forward's three calls and their nine tensors, a third of that for one.
 //
 //   forward   Q(x) [, Qt(x)], Q(w) [, Q(w)^T], y = Q(x) Q(w)^T
-//   backward  Q(e) and / or Qt(e), dx = Q(e) Q(w), dw = Qt(e)^T Qt(x)
+//   backward  Q(e) and / or Qt(e), dx = Q(e) Q(w), dw = Qt(e)^T Qt(x); the two products in one launch where that is quicker
 #include "common.cuh"
+#include "gemm_fp8.cuh"
 
 using namespace quartet;
 
@@ -86,7 +87,17 @@ extern "C" __attribute__((visibility("default"))) int quartet_linear_fp8_train_b
     uint8_t *et = dw ? workspace + L.et : nullptr, *ets = dw ? workspace + L.ets : nullptr;
     int rc = quartet_quant_fp8(e, e_dtype, M, N, fmt, 0, ec, es, et, ets, stream);
     if (rc) return rc;
-    if (dx && (rc = quartet_gemm_fp8_tn(ec, es, fmt, saved + S.wt, saved + S.wts, QUARTET_E4M3, M, K, pad128(N), 1.0f, dx, dx_dtype, ldx, stream))) return rc;
-    if (dw) return quartet_gemm_fp8_tn(et, ets, fmt, saved + S.xt, saved + S.xts, QUARTET_E4M3, N, K, pad128(M), 1.0f, dw, dw_dtype, ldw, stream);
-    return QUARTET_OK;
+    if (dx && dw) {
+        // neither depends on the other (everything that the single entry checks has been checked above)
+        if ((rc = bind_context_of(saved)) || (rc = check_device())) return rc;
+        Fp8Product x{ec, saved + S.wt, {}}, y{et, saved + S.xt, {}};
+        x.g.a_sf = es, x.g.b_sf = saved + S.wts, x.g.M = M, x.g.N = K, x.g.ldd = ldx, x.g.k_chunks = (int)(pad128(N) / 128);
+        x.g.d = dx, x.g.d_f32 = dx_dtype == QUARTET_F32;
+        y.g.a_sf = ets, y.g.b_sf = saved + S.xts, y.g.M = N, y.g.N = K, y.g.ldd = ldw, y.g.k_chunks = (int)(pad128(M) / 128);
+        y.g.d = dw, y.g.d_f32 = dw_dtype == QUARTET_F32;
+        x.g.a_e5m2 = y.g.a_e5m2 = fmt, x.g.alpha = y.g.alpha = 1.0f;
+        return product_two(x, y, static_cast<cudaStream_t>(stream));
+    }
+    if (dx) return quartet_gemm_fp8_tn(ec, es, fmt, saved + S.wt, saved + S.wts, QUARTET_E4M3, M, K, pad128(N), 1.0f, dx, dx_dtype, ldx, stream);
+    return quartet_gemm_fp8_tn(et, ets, fmt, saved + S.xt, saved + S.xts, QUARTET_E4M3, N, K, pad128(M), 1.0f, dw, dw_dtype, ldw, stream);
 }

@@ -248,6 +248,26 @@ def test_products_repeat_bit_for_bit(ops):
         assert all(torch.equal(first, ops.gemm_fp8_tn(ac, asf, bc, bsf, out_dtype=torch.float32)) for _ in range(5))
 
 
+@pytest.mark.parametrize("M,K,N", [(65, 64, 300), (128, 256, 5000), (300, 4000, 100), (1000, 700, 900), (2050, 515, 1030), (4096, 640, 1920), (300, 2600, 2600),
+                                   (513, 8000, 257), (4100, 100, 4100)])
+@pytest.mark.parametrize("gd", [E4M3, E5M2])
+def test_both_gradients_equal_each_alone(ops, M, K, N, gd):
+    """The two products of a backward pass, which may share a launch, against each by itself (another form may add in another order)."""
+    x, w, e = torch.randn(M, K, device="cuda"), torch.randn(N, K, device="cuda") * 0.05, torch.randn(M, N, device="cuda").bfloat16()
+    _, saved = ops.fp8_linear_fwd(x, w, True, True, torch.bfloat16)
+    both = ops.fp8_linear_bwd(e, saved, K, gd, torch.float32, torch.bfloat16, True, True, True, True)
+    dx, _ = ops.fp8_linear_bwd(e, saved, K, gd, torch.float32, torch.bfloat16, True, False, True, True)
+    _, dw = ops.fp8_linear_bwd(e, saved, K, gd, torch.float32, torch.bfloat16, False, True, True, True)
+    ev, et = (ops.dequant_fp8(c, s, n).double().abs() for c, s, n in ((*ops.quant_fp8(e, gd)[:2], N), (*ops.quant_fp8(e.T.contiguous(), gd)[:2], M)))
+    wv, xt = ops.dequant_fp8(*ops.quant_fp8(w, square=True)[:2], K).double().abs(), ops.dequant_fp8(*ops.quant_fp8(x.T.contiguous())[:2], M).double().abs()
+    for got, want, absum, k in ((both[0], dx, ev @ wv, N), (both[1], dw, et @ xt.T, M)):
+        lim = 2 * fo.pad128(k) * 2.0 ** -23 * absum
+        lim = lim + torch.finfo(got.dtype).eps * (want.double().abs() + lim) + 1e-40
+        assert bool(((got.double() - want.double()).abs() <= lim).all())
+    again = ops.fp8_linear_bwd(e, saved, K, gd, torch.float32, torch.bfloat16, True, True, True, True)
+    assert torch.equal(again[0], both[0]) and torch.equal(again[1], both[1]) and ops.device_status() == 0
+
+
 @pytest.mark.parametrize("M,K,N", [(1, 128, 128), (7, 100, 65), (130, 640, 1000), (256, 384, 512), (513, 257, 640)])
 @pytest.mark.parametrize("xd,wd,gd", [(torch.bfloat16, torch.float32, E4M3), (torch.float32, torch.float32, E5M2), (torch.bfloat16, torch.bfloat16, E5M2)])
 def test_layer_and_its_gradients(ops, M, K, N, xd, wd, gd):
