@@ -63,6 +63,30 @@ class WgradReduceScatter:
         return out
 
 
+class ExchangeCount:
+    """Exchanges that a sink was given, and how many of them wait() has joined; the same on every rank."""
+
+    def __init__(self):
+        self.submitted = self.joined = 0
+
+
+class ShardRecord:
+    """Which exchange a weight's `grad_shard` is to come from, and how many the sink had been given when it was last clipped."""
+
+    def __init__(self, count: ExchangeCount):
+        self.count, self.serial, self.clipped_at = count, count.submitted, None
+
+    @property
+    def in_flight(self) -> bool:
+        # not "has the sum been issued yet": that differs from rank to rank, and whoever asks may have a collective to make next
+        return self.serial > self.count.joined
+
+    @property
+    def stale(self) -> bool:
+        """Clipped before, and exchanges of a later step have followed in which the weight took no part."""
+        return self.clipped_at is not None and self.count.submitted > self.clipped_at
+
+
 class PeerSetupError(RuntimeError):
     """Raised on EVERY rank when any rank failed to allocate or map the receive buffers."""
 
@@ -79,8 +103,9 @@ class PeerWgradScatter:
 
     Attach with `layer.wgrad_sink = sink`; the layer's backward then returns no dense weight gradient
     and the averaged shard (rows [rank*N/world, (rank+1)*N/world)) is found in `layer.weight.grad_shard`
-    after `sink.wait()`.  Call `wait()` at least once per step: the two receive buffers of a layer alternate
-    from use to use, and a buffer is reused only after the sum of its previous contents has been issued.
+    after `sink.wait()`.  Call `wait()` at least once per step, before the shards are clipped or used: the two receive
+    buffers of a layer alternate from use to use, and a buffer is reused only after the sum of its previous contents has
+    been issued.  A shard stays where it is until the layer's next exchange replaces it; zero_grad() does not know it.
     """
 
     MAX_WORLD = 8
@@ -106,6 +131,7 @@ class PeerWgradScatter:
         self.plans = {}
         self.pending = []
         self.unreduced = []   # exchanges in flight: (weight, plan, parity, event "all ranks' rows have landed")
+        self.count = ExchangeCount()
         self.lag = 1          # how many exchanges may stay in flight before the compute stream is made to wait for the oldest
 
     def accepts(self, rows: int, cols: int, dtype: torch.dtype) -> bool:
@@ -205,6 +231,8 @@ class PeerWgradScatter:
         # by: on a side stream it would run beside the persistent GEMM, get a handful of SMs and delay the CTAs of
         # the next GEMM launch that need them.
         self.unreduced.append((weight, plan, parity, arrived))
+        self.count.submitted += 1
+        weight.grad_shard_record = ShardRecord(self.count)
         return None
 
     def _reduce_ready(self, block: bool = False):
@@ -224,6 +252,7 @@ class PeerWgradScatter:
     def wait(self):
         """Joins every exchange submitted so far; returns the owned, averaged shards in submission order."""
         self._reduce_ready(block=True)
+        self.count.joined = self.count.submitted
         self.ops.raise_on_fault("weight-gradient exchange")  # only with QUARTET_CHECK_FAULTS=1
         out, self.pending = self.pending, []
         return out
