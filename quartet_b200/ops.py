@@ -8,6 +8,7 @@ import os
 from array import array
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -70,6 +71,22 @@ def _need_cuda(*ts):
             raise ValueError("tensors must live on a CUDA device")
         if t is not None and not t.is_contiguous():
             raise ValueError("tensors must be contiguous")
+
+
+def forward_mode() -> bool:
+    """Whether a level of forward-mode differentiation is open.  Its inputs have no requires_grad: a call that reads their memory itself has to
+    ask for them here, or their tangents are lost without a word."""
+    return getattr(_forward_ad, "_current_level", 0) >= 0
+
+
+def eagerly(fn, *args):
+    """fn(*args) outside any graph being compiled: a compiler calls an autograd function's forward without its forward-mode derivative."""
+    # (disable() loads the compiler, some four seconds, so it is called here and not as a decorator)
+    return torch.compiler.disable(fn)(*args)
+
+
+def has_tangent(*ts) -> bool:
+    return forward_mode() and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def sf_bytes(rows: int, cols: int) -> int:

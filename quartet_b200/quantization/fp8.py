@@ -34,7 +34,7 @@ class _Fp8LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, e):
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or ops.has_tangent(e):
             raise RuntimeError("fp8_linear is not differentiable twice")
         need_dx, need_dw = ctx.needs_input_grad[:2]
         if not (need_dx or need_dw):
@@ -59,9 +59,12 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, grad_dtype: torch.dtype
         raise ValueError("x and weight must live on one CUDA device")
     ops._f8(grad_dtype)
     out_dtype = out_dtype or _out_dtype(x, x.dtype)
-    if torch.compiler.is_compiling():
-        need = torch.is_grad_enabled()
-        return torch.ops.quartet_b200.fp8_linear_fwd(x, weight, grad_dtype, out_dtype, need and x.requires_grad, need and weight.requires_grad)[0]
+    if (torch.compiler.is_compiling() or torch.jit.is_tracing()) and not ops.forward_mode():
+        # a compiled graph is guarded on what needs a gradient; a trace is not, and may be called with other inputs, so it keeps both transposes
+        need_dx, need_dw = (True, True) if torch.jit.is_tracing() else [torch.is_grad_enabled() and t.requires_grad for t in (x, weight)]
+        return torch.ops.quartet_b200.fp8_linear_fwd(x, weight, grad_dtype, out_dtype, need_dx, need_dw)[0]
+    if ops.forward_mode():  # the function has no such derivative, and says so where an input has a tangent
+        return ops.eagerly(_Fp8LinearFn.apply, x, weight, grad_dtype, out_dtype)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _Fp8LinearFn.apply(x, weight, grad_dtype, out_dtype)
     return _forward(x, weight, False, False, out_dtype)[0]  # nothing is kept, so neither transpose is made

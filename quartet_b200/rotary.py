@@ -5,7 +5,7 @@ whose pairs are interleaved).
     q, k = apply_rotary(q, k, inv_freq, positions)                      # [batch, tokens, heads, d], any strides
     q, k, v = rotary_qkv(qkv, n_head, n_kv_head, inv_freq)              # packed projection -> heads, one pass over memory
 
-Both are differentiable; the backward of rotary_qkv writes the packed gradient that the projection's backward reads.
+Both are differentiable, in reverse and in forward mode; the backward of rotary_qkv writes the packed gradient that the projection's backward reads.
 """
 from __future__ import annotations
 
@@ -85,6 +85,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, inv_freq, positions, offset, interleaved, scale, inverse):
         ctx.save_for_backward(inv_freq, positions)
+        ctx.save_for_forward(inv_freq, positions)
         ctx.args = (offset, interleaved, scale, inverse)
         ctx.set_materialize_grads(False)
         if k is None:
@@ -99,11 +100,28 @@ class _Rotary(torch.autograd.Function):
         gs = ([dq] if need_q else []) + ([dk] if need_k else [])
         if not gs:
             return (None,) * 8
-        if torch.is_grad_enabled():  # create_graph: the gradient is a rotation too
-            outs = _Rotary.apply(gs[0], gs[1] if len(gs) == 2 else None, inv_freq, positions, offset, interleaved, scale, not inverse)
+        if torch.is_grad_enabled() or ops.forward_mode():  # create_graph, or tangents: the gradient is a rotation too
+            outs = _turn_by_mode(gs[0], gs[1] if len(gs) == 2 else None, inv_freq, positions, offset, interleaved, scale, not inverse)
         else:
             outs = _turn(gs, inv_freq, positions, offset, interleaved, scale, not inverse)
         return outs[0] if need_q else None, outs[-1 if len(gs) == 2 else 0] if need_k else None, None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *unused):
+        inv_freq, positions = ctx.saved_tensors
+        return _Rotary.apply(tq, None, inv_freq, positions, *ctx.args)  # linear: the tangent turns alike (k: _turn_by_mode sends it alone)
+
+
+def _turn_by_mode(q, k, *args):
+    """_Rotary.apply; with a level of forward mode open each tensor by itself, as either may be without a tangent."""
+    if k is None or not ops.forward_mode():
+        return _Rotary.apply(q, k, *args)
+    return _Rotary.apply(q, None, *args)[0], _Rotary.apply(k, None, *args)[0]
+
+
+def _recording() -> bool:
+    """Whether the call is being put into a graph (compiled, exported, traced), where only registered operators are seen."""
+    return (torch.compiler.is_compiling() or torch.jit.is_tracing()) and not ops.forward_mode()
 
 
 def _check_heads(x, what):
@@ -117,10 +135,12 @@ def apply_rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=True, 
     _check_heads(q, "q")
     if k is not None:
         _check_heads(k, "k")
-    if torch.compiler.is_compiling():
+    if _recording():
         turn = torch.ops.quartet_b200.rotary
         return (turn(q, inv_freq, positions, offset, interleaved, scale, False),
                 None if k is None else turn(k, inv_freq, positions, offset, interleaved, scale, False))
+    if ops.forward_mode():
+        return ops.eagerly(_turn_by_mode, q, k, inv_freq, positions, offset, interleaved, scale, False)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, inv_freq, positions, offset, interleaved, scale, False)
     if k is None:
@@ -132,15 +152,20 @@ class _RotaryQKV(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major):
         ctx.save_for_backward(inv_freq, positions)
-        ctx.args = (offset, interleaved, scale, head_major)
+        ctx.save_for_forward(inv_freq, positions)
+        ctx.heads, ctx.args = (n_head, n_kv_head), (offset, interleaved, scale, head_major)
         return torch_ops.split_heads(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
 
     @staticmethod
     def backward(ctx, dq, dk, dv):
         inv_freq, positions = ctx.saved_tensors
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or ops.has_tangent(dq, dk, dv):
             raise RuntimeError("rotary_qkv is not differentiable twice: use apply_rotary under create_graph")
         return torch_ops.join_heads(dq, dk, dv, inv_freq, positions, *ctx.args), None, None, None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, t, *unused):
+        return _RotaryQKV.apply(t, *ctx.heads, *ctx.saved_tensors, *ctx.args)
 
 
 def rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions=None, *, offset=0, interleaved=True, scale=1.0, head_major=True):
@@ -148,8 +173,10 @@ def rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions=None, *, offset=0, in
     (head_major, what scaled_dot_product_attention takes) or [batch, tokens, heads, d], each contiguous."""
     if qkv.dim() != 3 or n_head < 1 or n_kv_head < 1 or qkv.shape[2] % (n_head + 2 * n_kv_head) or qkv.shape[2] == 0:
         raise ValueError("qkv must be [batch, tokens, (n_head + 2 n_kv_head) * d]")
-    if torch.compiler.is_compiling():
+    if _recording():
         return torch.ops.quartet_b200.rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
+    if ops.forward_mode():
+        return ops.eagerly(_RotaryQKV.apply, qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
     if torch.is_grad_enabled() and qkv.requires_grad:
         return _RotaryQKV.apply(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
     return torch_ops.split_heads(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
