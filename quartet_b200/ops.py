@@ -519,7 +519,10 @@ def gemm_fp8_tn(a, a_sf, b, b_sf, alpha=1.0, out_dtype=torch.bfloat16):
 
 def linear_fp8(x, w, w_sf, out_dtype=None):
     """x [..., K] times a packed weight (codes [N, pad128(K)] and scales of quant_fp8(weight, square=True)) -> [..., N]: x is quantized in
-    blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear."""
+    blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear; not differentiable: an x that wants a gradient, or has a
+    tangent, is refused (call it under torch.no_grad() or on x.detach())."""
+    if (x.requires_grad and torch.is_grad_enabled()) or has_tangent(x):
+        raise RuntimeError("linear_fp8 has no derivative: call it under torch.no_grad() or on x.detach(), or use quantization.fp8_linear")
     _need_codes(w, w_sf, "linear_fp8")
     shape, dev = x.shape, w.device
     if len(shape) < 1 or shape[-1] < 1:

@@ -156,3 +156,13 @@ def test_trace_records_the_8_bit_layer(monkeypatch):
     f = torch.jit.trace(lambda a: fp8_linear(a, w), (torch.randn(2, 3, 8),))
     x = torch.randn(2, 3, 8)
     assert torch.equal(f(x), fp8_linear(x, w))
+
+
+def test_the_packed_form_refuses_what_it_cannot_differentiate():
+    x, w, sf = torch.randn(3, 256), torch.zeros(8, 256, dtype=torch.float8_e4m3fn), torch.zeros(ops.sf_bytes(8, 256), dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        ops.linear_fp8(x.clone().requires_grad_(), w, sf)
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="no derivative"):
+        ops.linear_fp8(fwad.make_dual(x, x), w, sf)
+    with torch.no_grad(), pytest.raises(ValueError):            # a leaf of a model that is served: only the device is wrong here
+        ops.linear_fp8(x.clone().requires_grad_(), w, sf)
