@@ -31,8 +31,12 @@ enum { A_CODES = 0, A_BF16 = 1, A_F32 = 2 };
 static inline int64_t gemv_pitch(int64_t pk) { return 2 * pk + 32; }
 bool gemv_fits(int64_t M, int64_t pk) { return M <= 8 && M * (gemv_pitch(pk) + pk / 32) <= 96 * 1024; }
 
-__device__ __forceinline__ float e8m0_value(uint32_t b) {
-    return __uint_as_float(b == 255u ? 0x7FC00000u : b == 0u ? 0x00400000u : b << 23);
+// acc + v 2^(w - 127) 2^(x - 127), NaN for a byte of 255.  The summed exponent is halved into two factors on the same side of one: what
+// lies between leaves fp32 only where the product does (below 2^-149 both are lost).
+__device__ __forceinline__ float scaled_add(float v, uint32_t w, uint32_t x, float acc) {
+    const uint32_t e = w + x, h = e >> 1, r = e - h;  // 0 .. 254 each: 2^(h - 127), 2^(r - 127), the least of them subnormal
+    const float a = __uint_as_float(max(w, x) == 255u ? 0x7FC00000u : max(h << 23, 0x00400000u)), b = __uint_as_float(max(r << 23, 0x00400000u));
+    return fmaf(v * a, b, acc);
 }
 
 template <bool E5M2>
@@ -206,26 +210,33 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
                 __syncwarp();
                 fill((int)s);  // the stage is in registers: its next copy may start
                 if (++s == GEMV_STAGES) s = 0, ph ^= 1;
-                // one scale for the whole chunk, as this library's quantizers write them, and none of them NaN
-                const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0) &&
-                                   max(max(w0, w1), max(x0, x1)) < 0xFF000000u;
-                if (__all_sync(0xFFFFFFFFu, block)) {
-                    // byte b in the exponent's place; for 0 the subnormal 2^-127
-                    const float sw0 = __uint_as_float(max((w0 >> 24) << 23, 0x00400000u)), sw1 = __uint_as_float(max((w1 >> 24) << 23, 0x00400000u));
-                    const float sx0 = __uint_as_float(max((x0 >> 24) << 23, 0x00400000u)), sx1 = __uint_as_float(max((x1 >> 24) << 23, 0x00400000u));
-                    acc[0] = fmaf(((cc[0][0] + cc[1][0]) + (cc[2][0] + cc[3][0])) * sw0, sx0, acc[0]);
-                    acc[1] = fmaf(((cc[0][1] + cc[1][1]) + (cc[2][1] + cc[3][1])) * sw0, sx1, acc[1]);
-                    acc[2] = fmaf(((cc[0][2] + cc[1][2]) + (cc[2][2] + cc[3][2])) * sw1, sx0, acc[2]);
-                    acc[3] = fmaf(((cc[0][3] + cc[1][3]) + (cc[2][3] + cc[3][3])) * sw1, sx1, acc[3]);
+                // Two factors 2^(b - 127) make one, 2^(w + x - 254), taken as a whole: either by itself may lead out of fp32 where the product is well
+                // inside.  One scale for the whole chunk, as this library's quantizers write them, and bytes of 64 .. 190, whose sums leave a normal factor:
+                const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0);
+                constexpr uint32_t LOW = 64u << 24, SPAN = 127u << 24, ONE = 127u << 23;
+                if (__all_sync(0xFFFFFFFFu, block && max(max(w0 - LOW, w1 - LOW), max(x0 - LOW, x1 - LOW)) < SPAN)) {
+                    const uint32_t f0 = (w0 >> 1) & 0x7F800000u, f1 = (w1 >> 1) & 0x7F800000u, g0 = (x0 >> 1) & 0x7F800000u, g1 = (x1 >> 1) & 0x7F800000u;
+                    const float s00 = __uint_as_float(f0 + g0 - ONE), s01 = __uint_as_float(f0 + g1 - ONE);
+                    const float s10 = __uint_as_float(f1 + g0 - ONE), s11 = __uint_as_float(f1 + g1 - ONE);
+                    acc[0] = fmaf((cc[0][0] + cc[1][0]) + (cc[2][0] + cc[3][0]), s00, acc[0]);
+                    acc[1] = fmaf((cc[0][1] + cc[1][1]) + (cc[2][1] + cc[3][1]), s01, acc[1]);
+                    acc[2] = fmaf((cc[0][2] + cc[1][2]) + (cc[2][2] + cc[3][2]), s10, acc[2]);
+                    acc[3] = fmaf((cc[0][3] + cc[1][3]) + (cc[2][3] + cc[3][3]), s11, acc[3]);
                 } else {
+                    // Rows of zeros (byte 0) come here too: a chunk under one scale then takes one step, not four.
+                    const bool whole = __all_sync(0xFFFFFFFFu, block);
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) cc[0][i] = (cc[0][i] + cc[1][i]) + (cc[2][i] + cc[3][i]);
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float sw0 = e8m0_value((w0 >> (8 * k)) & 255u), sw1 = e8m0_value((w1 >> (8 * k)) & 255u);
-                        const float sx0 = e8m0_value((x0 >> (8 * k)) & 255u), sx1 = e8m0_value((x1 >> (8 * k)) & 255u);
-                        acc[0] = fmaf(cc[k][0] * sw0, sx0, acc[0]);
-                        acc[1] = fmaf(cc[k][1] * sw0, sx1, acc[1]);
-                        acc[2] = fmaf(cc[k][2] * sw1, sx0, acc[2]);
-                        acc[3] = fmaf(cc[k][3] * sw1, sx1, acc[3]);
+                        if (k > 0 && whole) break;
+                        const uint32_t wb0 = (w0 >> (8 * k)) & 255u, wb1 = (w1 >> (8 * k)) & 255u, xb0 = (x0 >> (8 * k)) & 255u, xb1 = (x1 >> (8 * k)) & 255u;
+                        acc[0] = scaled_add(cc[k][0], wb0, xb0, acc[0]);
+                        acc[1] = scaled_add(cc[k][1], wb0, xb1, acc[1]);
+                        acc[2] = scaled_add(cc[k][2], wb1, xb0, acc[2]);
+                        acc[3] = scaled_add(cc[k][3], wb1, xb1, acc[3]);
                     }
                 }
             }
