@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(256) dequant_fp8_kernel(const uint8_t* __restr
         const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(codes + row * pitch + c));
         const int64_t r = row & 127;
         const uint32_t b = __ldg(sf + ((row >> 7) * (pitch >> 7) + (c >> 7)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + ((c >> 5) & 3));
-        const float s = (b == 255u ? __uint_as_float(0x7FC00000u) : b == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23)) * scale;
+        const float s = b == 255u ? __uint_as_float(0x7FC00000u) : b == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
         for (int k = 0; k < 4 && c + k < cols; ++k) {
             uint32_t h;
             const uint16_t two = (uint16_t)((w >> (8 * k)) & 0xFFu);
@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(256) dequant_fp8_kernel(const uint8_t* __restr
                 asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"(two));
             else
                 asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-            const float v = __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu))) * s;
+            // the code's own value first, which is exact: 2^e times the factor may leave fp32 or its normal range where the result is inside
+            const float v = __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu))) * s * scale;
             if (F32OUT)
                 static_cast<float*>(out)[row * cols + c + k] = v;
             else

@@ -77,3 +77,15 @@ def test_rows_of_zeros_beside_others(ops, M):
     exact = fo.values(x.cpu(), E4M3) @ fo.values(w.cpu(), E4M3, True).T
     s = fo.values(x.cpu(), E4M3).abs() @ fo.values(w.cpu(), E4M3, True).abs().T
     assert bool(((want.cpu().double() - exact).abs() <= 1024 * 2.0 ** -23 * s + exact.abs() * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_reading_back_with_a_factor_rounds_once(ops, dtype):
+    """code 2^(b - 127) scale, where the scale and the block's power of two alone leave fp32 or its normal range."""
+    codes = torch.tensor([2.0 ** -9, -3 * 2.0 ** -9, 2.0 ** -6, 1.125, 448.0, 0.0]).repeat(64)[:256].view(2, 128).to(E4M3)
+    for byte, scale in ((250, 1024.0), (254, 0.3), (0, 0.3), (1, 1e-3), (100, 3e38), (127, 1.1), (40, 7e-13)):
+        sf = _blocked32(torch.full((2, 4), byte, dtype=torch.uint8)).cuda()
+        got = ops.dequant_fp8(codes.cuda(), sf, scale=scale, dtype=dtype).cpu()
+        want = codes.double() * 2.0 ** (byte - 127) * torch.tensor(scale).double()      # the factor itself is fp32
+        f32 = want.float()                                                              # rounds, overflows and underflows as one product does
+        assert torch.equal(got, f32.to(dtype)), (byte, scale)
