@@ -489,17 +489,23 @@ def dequant_fp8(codes, sf, cols=None, scale=1.0, dtype=torch.float32):
     return out
 
 
-def _padded_out(rows, cols, dtype, dev):
-    """[rows, cols] whose rows start on 16-byte boundaries: a view of a wider buffer where cols does not fill one."""
+def _padded_out(lead, cols, dtype, dev):
+    """[*lead, cols] whose rows start on 16-byte boundaries, and their pitch in elements.  No view of another tensor, even where the rows are
+    padded: what an autograd function returns could not be changed in place otherwise."""
     per = 16 // dtype.itemsize
     pitch = (cols + per - 1) // per * per
-    out = torch.empty(rows, pitch, dtype=dtype, device=dev)
-    return (out if pitch == cols else out[:, :cols]), pitch
+    if pitch == cols:
+        return torch.empty(*lead, cols, dtype=dtype, device=dev), pitch
+    strides, step = [1], pitch
+    for n in reversed(lead):
+        strides.append(step)
+        step *= max(n, 1)
+    return torch.empty_strided((*lead, cols), strides[::-1], dtype=dtype, device=dev), pitch
 
 
 def gemm_fp8_tn(a, a_sf, b, b_sf, alpha=1.0, out_dtype=torch.bfloat16):
     """D[M, N] = alpha * A[M, K] . B[N, K]^T on 8-bit codes with blocked E8M0 scales, as quant_fp8 makes them.  Where a row of D is no
-    multiple of 16 bytes, D is a view of a buffer whose rows are."""
+    multiple of 16 bytes, D's rows are padded in memory so that they start on one."""
     _need_codes(a, a_sf, "gemm_fp8_tn (a)")
     _need_codes(b, b_sf, "gemm_fp8_tn (b)")
     (M, K), N = a.shape, b.shape[0]
@@ -510,7 +516,7 @@ def gemm_fp8_tn(a, a_sf, b, b_sf, alpha=1.0, out_dtype=torch.bfloat16):
     fa, fb, dd = _f8(a.dtype), _f8(b.dtype), _out_dt(out_dtype)
     if M == 0 or N == 0 or K == 0:
         return torch.zeros(M, N, dtype=out_dtype, device=a.device)
-    out, pitch = _padded_out(M, N, out_dtype, a.device)
+    out, pitch = _padded_out((M,), N, out_dtype, a.device)
     with _on(a.device):
         rc = _lib.load().quartet_gemm_fp8_tn(_ptr(a), _ptr(a_sf), fa, _ptr(b), _ptr(b_sf), fb, M, N, K, alpha, _ptr(out), dd, pitch, _stream())
     _lib.check(rc, "quartet_gemm_fp8_tn")
@@ -537,7 +543,7 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
     M = x.numel() // K
     dtype = out_dtype or x.dtype
     xd, wd, yd = _dt(x), _f8(w.dtype), _out_dt(dtype)
-    y, pitch = _padded_out(M, N, dtype, dev)
+    y, pitch = _padded_out(shape[:-1], N, dtype, dev)
     if M and N:
         lib = _lib.load()
         nbytes = lib.quartet_linear_fp8_workspace_bytes(M, K)
@@ -547,7 +553,7 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
                                         y.data_ptr(), yd, pitch, _stream())
         if rc:
             _lib.check(rc, "quartet_linear_fp8")
-    return y if len(shape) == 2 else y.view(*shape[:-1], N)
+    return y
 
 
 @functools.lru_cache(maxsize=4096)
@@ -557,19 +563,20 @@ def _fp8_train_bytes(M, N, K, need_dx, need_dw):
     return tuple(out)
 
 
-def fp8_linear_fwd(x2, w, need_dx, need_dw, out_dtype):
-    """x2 [M, K], w [N, K] -> (y [M, N], saved): the 8-bit layer's forward in one call; saved is what fp8_linear_bwd takes."""
-    _need_cuda(x2, w)
-    (M, K), N, dev = x2.shape, w.shape[0], x2.device
-    xd, wd, yd = _dt(x2), _dt(w), _out_dt(out_dtype)
-    y, pitch = _padded_out(M, N, out_dtype, dev)
+def fp8_linear_fwd(x, w, need_dx, need_dw, out_dtype):
+    """x [..., K], w [N, K] -> (y [..., N], saved): the 8-bit layer's forward in one call; saved is what fp8_linear_bwd takes."""
+    _need_cuda(x, w)
+    (N, K), dev = w.shape, x.device
+    M = x.numel() // K if K else x.shape[:-1].numel()
+    xd, wd, yd = _dt(x), _dt(w), _out_dt(out_dtype)
+    y, pitch = _padded_out(x.shape[:-1], N, out_dtype, dev)
     need_dx, need_dw = 1 if need_dx else 0, 1 if need_dw else 0
     if not (M and N and K):
         return y.zero_(), torch.empty(0, dtype=torch.uint8, device=dev)
     saved_bytes, work_bytes, _ = _fp8_train_bytes(M, N, K, need_dx, need_dw)
     saved, work = torch.empty(saved_bytes, dtype=torch.uint8, device=dev), torch.empty(work_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = _lib.load().quartet_linear_fp8_train_fwd(x2.data_ptr(), xd, w.data_ptr(), wd, M, N, K, need_dx, need_dw, saved.data_ptr() if saved_bytes else None,
+        rc = _lib.load().quartet_linear_fp8_train_fwd(x.data_ptr(), xd, w.data_ptr(), wd, M, N, K, need_dx, need_dw, saved.data_ptr() if saved_bytes else None,
                                                       work.data_ptr(), y.data_ptr(), yd, pitch, _stream())
     if rc:
         _lib.check(rc, "quartet_linear_fp8_train_fwd")
@@ -581,8 +588,8 @@ def fp8_linear_bwd(e2, saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw,
     _need_cuda(e2, saved)
     (M, N), dev = e2.shape, e2.device
     ed, fmt = _dt(e2), _f8(grad_dtype)
-    dx, ldx = _padded_out(M, K, x_dtype, dev) if need_dx else (None, 0)
-    dw, ldw = _padded_out(N, K, w_dtype, dev) if need_dw else (None, 0)
+    dx, ldx = _padded_out((M,), K, x_dtype, dev) if need_dx else (None, 0)
+    dw, ldw = _padded_out((N,), K, w_dtype, dev) if need_dw else (None, 0)
     if not (M and N and K):
         return None if dx is None else dx.zero_(), None if dw is None else dw.zero_()
     work = torch.empty(_fp8_train_bytes(M, N, K, 1 if need_dx else 0, 1 if need_dw else 0)[2], dtype=torch.uint8, device=dev)

@@ -18,9 +18,7 @@ from .producers import _out_dtype
 
 
 def _forward(x, w, need_dx, need_dw, out_dtype):
-    x2 = x if x.dim() == 2 else x.reshape(-1, w.shape[1])
-    y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0]), saved
+    return ops.fp8_linear_fwd(x if x.is_contiguous() else x.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
 
 
 class _Fp8LinearFn(torch.autograd.Function):

@@ -552,9 +552,8 @@ torch.library.register_autograd("quartet_b200::rotary_qkv", _rotary_qkv_backward
 @torch.library.custom_op("quartet_b200::fp8_linear_fwd", mutates_args=())
 def fp8_linear_fwd(x: Tensor, w: Tensor, grad_dtype: torch.dtype, out_dtype: torch.dtype, need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
     """y = Q(x) Q(w)^T and what its backward needs: codes and scales of x and w transposed, as one buffer."""
-    x2 = x.reshape(-1, w.shape[1])
-    y, saved = ops.fp8_linear_fwd(x2 if x2.is_contiguous() else x2.contiguous(), w if w.is_contiguous() else w.contiguous(), need_dx, need_dw, out_dtype)
-    return y.reshape(*x.shape[:-1], w.shape[0]).contiguous(), saved
+    y, saved = ops.fp8_linear_fwd(x.contiguous(), w.contiguous(), need_dx, need_dw, out_dtype)
+    return y.contiguous(), saved
 
 
 def _pad256(n: int) -> int:

@@ -89,3 +89,18 @@ def test_reading_back_with_a_factor_rounds_once(ops, dtype):
         want = codes.double() * 2.0 ** (byte - 127) * torch.tensor(scale).double()      # the factor itself is fp32
         f32 = want.float()                                                              # rounds, overflows and underflows as one product does
         assert torch.equal(got, f32.to(dtype)), (byte, scale)
+
+
+@pytest.mark.parametrize("n", [64, 77])
+def test_results_changed_in_place_before_the_backward(ops, n):
+    from quartet_b200.quantization import fp8_linear
+
+    x, w = torch.randn(2, 9, 200, device="cuda"), torch.randn(n, 200, device="cuda") * 0.05
+    grads = []
+    for inplace in (False, True):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = fp8_linear(a, b)
+        y = y.mul_(0.5).add_(1.0) if inplace else y * 0.5 + 1.0
+        y.square().sum().backward()
+        grads.append((y.detach(), a.grad, b.grad))
+    assert all(torch.equal(u, v) for u, v in zip(*grads))
