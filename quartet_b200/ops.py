@@ -566,6 +566,8 @@ def _fp8_train_bytes(M, N, K, need_dx, need_dw):
 def fp8_linear_fwd(x, w, need_dx, need_dw, out_dtype):
     """x [..., K], w [N, K] -> (y [..., N], saved): the 8-bit layer's forward in one call; saved is what fp8_linear_bwd takes."""
     _need_cuda(x, w)
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1] or w.device != x.device:
+        raise ValueError(f"x [..., K] and w [N, K] on one device are needed, not {tuple(x.shape)} and {tuple(w.shape)}")
     (N, K), dev = w.shape, x.device
     M = x.numel() // K if K else x.shape[:-1].numel()
     xd, wd, yd = _dt(x), _dt(w), _out_dt(out_dtype)
@@ -586,8 +588,13 @@ def fp8_linear_fwd(x, w, need_dx, need_dw, out_dtype):
 def fp8_linear_bwd(e2, saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw, saved_dx, saved_dw):
     """e2 [M, N] and the forward's saved buffer (made with need_dx = saved_dx, need_dw = saved_dw) -> (dx [M, K] | None, dw [N, K] | None)."""
     _need_cuda(e2, saved)
+    if e2.dim() != 2 or saved.device != e2.device:
+        raise ValueError("e [M, N] and the kept buffer on one device are needed")
     (M, N), dev = e2.shape, e2.device
     ed, fmt = _dt(e2), _f8(grad_dtype)
+    # the library sees an address only: the buffer's size is what tells whether it was kept for these extents
+    if M and N and K and (saved.dtype != torch.uint8 or saved.numel() != _fp8_train_bytes(M, N, K, 1 if saved_dx else 0, 1 if saved_dw else 0)[0]):
+        raise ValueError(f"the kept buffer does not belong to a layer of {M} x {N}, K {K}")
     dx, ldx = _padded_out((M,), K, x_dtype, dev) if need_dx else (None, 0)
     dw, ldw = _padded_out((N,), K, w_dtype, dev) if need_dw else (None, 0)
     if not (M and N and K):

@@ -45,3 +45,23 @@ def test_results_can_be_changed_in_place(shape, n):
         assert fp8_linear(x, w).shape == (*shape[:-1], n)
     # rows start on 16-byte boundaries
     assert y.numel() == 0 or all(s % 4 == 0 for s, extent in zip(y.stride()[:-1], y.shape) if extent > 1)
+
+
+def test_operands_that_do_not_belong_together_are_refused(monkeypatch):
+    """What the library cannot see from addresses: extents that differ, and a kept buffer that is not this backward's."""
+    x, w, e = torch.zeros(40, 256), torch.zeros(64, 256), torch.zeros(40, 64)
+    for a, b in ((x, torch.zeros(64, 128)), (torch.zeros(40, 300), w), (x, w[0]), (torch.zeros(()), w)):
+        with pytest.raises(ValueError):
+            ops.fp8_linear_fwd(a, b, True, True, torch.float32)
+    with pytest.raises(ValueError):
+        ops.fp8_linear_fwd(x, w, True, True, torch.float16)
+    y, saved = ops.fp8_linear_fwd(x, w, True, True, torch.float32)
+    back = lambda e=e, s=saved, K=256, dx=True, dw=True, sx=True, sw=True: ops.fp8_linear_bwd(e, s, K, torch.float8_e4m3fn, torch.float32, torch.float32, dx, dw, sx, sw)  # noqa: E731
+    assert [t.shape for t in back()] == [(40, 256), (64, 256)]
+    only = ops.fp8_linear_fwd(x, w, False, True, torch.float32)[1]
+    assert back(s=only, dx=False, sx=False)[0] is None
+    for bad in (dict(s=saved[:-1]), dict(s=only), dict(s=saved.float()), dict(e=torch.zeros(300, 64)), dict(e=torch.zeros(40, 200)), dict(K=1024), dict(e=e[0]),
+                dict(s=torch.empty(0, dtype=torch.uint8)), dict(sx=False, dx=False)):
+        with pytest.raises(ValueError):
+            back(**bad)
+    assert back(e=torch.zeros(0, 64), s=torch.empty(0, dtype=torch.uint8))[1].shape == (64, 256)
