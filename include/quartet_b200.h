@@ -288,7 +288,8 @@ int quartet_linear_fp8_train_bwd(const void* e, int e_dtype, int64_t M, int64_t 
  * layout; 0: pairs (i, i + rot / 2).  inverse 1: by the negative angle (the gradient).
  * n_seg (1..3) tensors share the launch: segment g is src[g] -> dst[g] with heads[g] heads, element strides strides6[6 g ..] = {src batch,
  * src token, src head, dst batch, dst token, dst head}, values of a head adjacent; rotate[g] 0 copies it (v).  The five arrays are
- * HOST arrays.  A dst may be its own src with the same strides; otherwise they must not overlap.
+ * HOST arrays.  A dst may be its own src with the same strides; any other sharing of memory by a dst, with a src, another dst or itself (an
+ * expanded view), is refused, and so is a layout so irregular that it cannot be ruled out.
  * pos: NULL (token t is at offset + t), or int32 / int64 (pos_i64) with strides for batch and token.  inv_freq: double [rot / 2].
  * rot even, <= min(d, 512); batch * tokens < 2^31.
  */

@@ -12,6 +12,8 @@
 // them in registers and walks the heads in batches, the next batch's loads under way while one is turned and stored.  Where there are few
 // tokens a thread takes every split-th head, and the threads of a token share its pairs through shared memory.
 // Bound by memory: each value is read and written once.
+#include <algorithm>
+
 #include "common.cuh"
 #include "quant_math.cuh"
 
@@ -218,6 +220,113 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_consta
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// Whether two of the strided tensors of a launch share memory.  A tensor is the set of addresses base + sum over its axes of index * stride; two of
+// them meet where the difference of their bases is a sum over all axes of coefficient * stride, each coefficient between limits.  That is
+// searched axis by axis, largest stride first: what the axes behind can still reach leaves one or two coefficients of each to try where the axes
+// nest, as those of views of one buffer do.
+// (A launch is a few microseconds of host time: ranges that lie apart and axes that nest are told without a search, half of one in all.)
+struct RotSpan {
+    int64_t base, n[4], st[4];  // bytes; batch, token, head, value, an axis of one entry with stride 0
+    int64_t reach;              // last value's address - first's
+};
+struct RotAxis {
+    int64_t st, lo, hi;
+};
+constexpr int ROT_SEARCH = 4096;  // coefficients tried before the answer is "cannot tell"
+
+static RotSpan rot_span(const void* p, int eb, int64_t batch, int64_t tokens, int64_t heads, int64_t d, const int64_t* st3) {
+    RotSpan s{(int64_t)reinterpret_cast<uintptr_t>(p), {batch, tokens, heads, d}, {st3[0] * eb, st3[1] * eb, st3[2] * eb, eb}, 0};
+    for (int i = 0; i < 4; ++i) {
+        if (s.n[i] == 1) s.st[i] = 0;
+        if (s.st[i] < 0) s.base += (s.n[i] - 1) * s.st[i], s.st[i] = -s.st[i];
+        s.reach += (s.n[i] - 1) * s.st[i];
+    }
+    return s;
+}
+static inline int64_t floor_div(int64_t a, int64_t b) {
+    if (a >= 0 && a < b) return 0;
+    if (a < 0 && a >= -b) return -1;
+    const int64_t q = a / b;
+    return q - (q * b > a);
+}
+
+// 1: some choice of coefficients from axis i on adds up to `left` (`moved`: a choice of another address than a tensor's with itself), 0: none, -1: not
+// found in ROT_SEARCH steps.  lo, hi: what the axes from i on reach.
+static int rot_meets(const RotAxis* ax, int n, int i, int64_t left, int64_t lo, int64_t hi, bool moved, int& budget) {
+    if (i == n) return left == 0 && moved;
+    lo -= ax[i].lo * ax[i].st, hi -= ax[i].hi * ax[i].st;
+    const int64_t first = std::max(ax[i].lo, -floor_div(hi - left, ax[i].st)), last = std::min(ax[i].hi, floor_div(left - lo, ax[i].st));
+    for (int64_t c = first; c <= last; ++c) {
+        if (--budget < 0) return -1;
+        const int r = rot_meets(ax, n, i + 1, left - c * ax[i].st, lo, hi, moved || c != 0, budget);
+        if (r) return r;
+    }
+    return 0;
+}
+static int rot_search(RotAxis* ax, int n, int64_t left, bool moved) {
+    std::sort(ax, ax + n, [](const RotAxis& x, const RotAxis& y) { return x.st > y.st; });
+    int64_t lo = 0, hi = 0;
+    for (int k = 0; k < n; ++k) lo += ax[k].lo * ax[k].st, hi += ax[k].hi * ax[k].st;
+    int budget = ROT_SEARCH;
+    return rot_meets(ax, n, 0, left, lo, hi, moved, budget);
+}
+// Whether two indexes of one tensor share an address.
+static int rot_folds(const RotSpan& a) {
+    int64_t inner = -1;  // axes that nest: every stride is more than all smaller ones reach together
+    int order[4], n = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (a.n[i] == 1) continue;
+        if (a.st[i] == 0) return 1;
+        int k = n++;
+        for (; k > 0 && a.st[order[k - 1]] > a.st[i]; --k) order[k] = order[k - 1];
+        order[k] = i;
+    }
+    bool nest = true;
+    for (int k = 0; k < n && nest; ++k) {
+        nest = a.st[order[k]] > inner;
+        inner = std::max<int64_t>(inner, 0) + (a.n[order[k]] - 1) * a.st[order[k]];
+    }
+    if (nest) return 0;
+    RotAxis ax[4];
+    for (int k = 0; k < n; ++k) {
+        if (k && a.st[order[k]] == a.st[order[k - 1]]) return 1;
+        ax[k] = RotAxis{a.st[order[k]], 1 - a.n[order[k]], a.n[order[k]] - 1};
+    }
+    return rot_search(ax, n, 0, false);
+}
+// Whether two tensors share an address.
+static int rot_overlap(const RotSpan& a, const RotSpan& b) {
+    if (a.base > b.base + b.reach || b.base > a.base + a.reach) return 0;
+    RotAxis ax[8];
+    int n = 0;
+    auto axis = [&](int64_t st, int64_t lo, int64_t hi) {
+        for (int k = 0; k < n; ++k)
+            if (ax[k].st == st) {
+                ax[k].lo += lo, ax[k].hi += hi;
+                return;
+            }
+        ax[n++] = RotAxis{st, lo, hi};
+    };
+    for (int i = 0; i < 4; ++i) {
+        if (a.st[i]) axis(a.st[i], 0, a.n[i] - 1);
+        if (b.st[i]) axis(b.st[i], 1 - b.n[i], 0);
+    }
+    return rot_search(ax, n, b.base - a.base, true);
+}
+// Every value is read by one thread and written by another, in no order: a dst may be its own src as a whole and nothing else's, nor hold one
+// value twice.
+static int refuse_rotary_overlap(int n_seg, const RotSpan* src, const RotSpan* dst) {
+    auto same = [](const RotSpan& a, const RotSpan& b) { return a.base == b.base && std::equal(a.st, a.st + 4, b.st); };
+    for (int g = 0; g < n_seg; ++g) {
+        if (rot_folds(dst[g])) return fail(QUARTET_E_ARG, "dst %d holds several values at one address", g);
+        for (int h = 0; h < n_seg; ++h) {
+            if (h < g && rot_overlap(dst[g], dst[h])) return fail(QUARTET_E_ARG, "dst %d and dst %d share memory", h, g);
+            if (!(g == h && same(dst[g], src[h])) && rot_overlap(dst[g], src[h])) return fail(QUARTET_E_ARG, "dst %d shares memory with src %d", g, h);
+        }
+    }
+    return QUARTET_OK;
+}
+
 template <bool F32, int BYTES>
 static int launch_rotary(RotParams p, bool interleaved, cudaStream_t s) {
     int rc, sms = 0, heads = 1;
@@ -260,6 +369,7 @@ extern "C" __attribute__((visibility("default"))) int quartet_rotary(int n_seg, 
     const bool f32 = dtype == QUARTET_F32;
     const int eb = f32 ? 4 : 2;
     RotParams p{};
+    RotSpan srcs[ROT_MAX_SEGS], dsts[ROT_MAX_SEGS];
     // every address that a thread forms is a sum of these: their common power of two is how much it may move at once
     uint64_t bits = 16 | (uint64_t)d * eb | (uint64_t)(interleaved ? rot : rot / 2) * eb;
     for (int g = 0; g < n_seg; ++g) {
@@ -270,12 +380,14 @@ extern "C" __attribute__((visibility("default"))) int quartet_rotary(int n_seg, 
             return fail(QUARTET_E_ALIGN, "segment %d is not aligned to its type", g);
         bits |= reinterpret_cast<uintptr_t>(src[g]) | reinterpret_cast<uintptr_t>(dst[g]);
         for (int k = 0; k < 6; ++k) bits |= (uint64_t)st[k] * (uint64_t)eb;
+        srcs[g] = rot_span(src[g], eb, batch, tokens, heads[g], d, st), dsts[g] = rot_span(dst[g], eb, batch, tokens, heads[g], d, st + 3);
         p.seg[g] = RotSeg{src[g], dst[g], st[0], st[1], st[2], st[3], st[4], st[5], heads[g], rotate[g] != 0};
     }
+    int rc = refuse_rotary_overlap(n_seg, srcs, dsts);
+    if (rc) return rc;
     if (reinterpret_cast<uintptr_t>(inv_freq) & 7u) return fail(QUARTET_E_ALIGN, "inv_freq must be 8-byte aligned");
     if (pos && (reinterpret_cast<uintptr_t>(pos) & (pos_i64 ? 7u : 3u))) return fail(QUARTET_E_ALIGN, "pos must be aligned to its type");
-    int rc = bind_context_of(src[0]);
-    if (rc) return rc;
+    if ((rc = bind_context_of(src[0]))) return rc;
     if ((rc = check_device())) return rc;
     p.n_seg = n_seg, p.d = (int)d, p.rot = (int)rot, p.T = tokens;
     p.pos = pos, p.pos_i64 = pos_i64, p.pos_b = pos_stride_b, p.pos_t = pos_stride_t, p.offset = offset;

@@ -615,7 +615,7 @@ def fp8_linear_bwd(e2, saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw,
 def rotary(segments, inv_freq, positions=None, offset=0, interleaved=True, scale=1.0, inverse=False):
     """Turns (or copies) up to three tensors in one launch.  segments: (src, dst, rotate), src and dst [batch, tokens, heads, d] views of any
     strides whose last axis is contiguous.  positions: int32 / int64 [tokens] or [batch, tokens], or None for offset, offset + 1, ...
-    inv_freq: float64 [rot / 2].  A dst may be its own src; otherwise they must not overlap."""
+    inv_freq: float64 [rot / 2].  A dst may be its own src; one that shares memory with anything else, or with itself, is refused."""
     x0 = segments[0][0]
     B, T, _, d = x0.shape
     dev, dtype = x0.device, x0.dtype

@@ -195,3 +195,22 @@ def test_gradient_of_the_gradient(R):
     qkv = torch.randn(1, 4, 3 * 16, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(R.rotary_qkv(qkv, 1, 1, inv)[0].sum(), (qkv,), create_graph=True)
+
+
+def test_destinations_that_share_memory_are_refused(R):
+    from quartet_b200 import ops
+
+    inv, _ = R.rotary_frequencies(64, device="cuda")
+    buf = torch.randn(2, 5, 12, 64, device="cuda")
+    q, k = buf[:, :, :4], buf[:, :, 4:8]
+    fresh = torch.empty(2, 5, 4, 64, device="cuda")
+    want = R.apply_rotary(q, None, inv)[0]
+    bad = [[(q, buf[:, :, 1:5], True)], [(q, fresh[:, :, :1].expand(2, 5, 4, 64), True)], [(q, fresh, True), (k, fresh, True)], [(q, k, True), (k, fresh, True)],
+           [(q, buf.view(-1)[1:2 * 5 * 4 * 64 + 1].view(2, 5, 4, 64), True)]]
+    kept = buf.clone()
+    for segments in bad:
+        with pytest.raises(ValueError, match="share|one address"):
+            ops.rotary(segments, inv)
+    assert torch.equal(buf, kept)
+    ops.rotary([(q, buf[:, :, 8:], True), (k, k, True)], inv)                # disjoint parts of one buffer, one of them in place
+    assert torch.equal(buf[:, :, 8:], want) and torch.equal(k, R.apply_rotary(kept[:, :, 4:8], None, inv)[0])
