@@ -553,20 +553,29 @@ torch.library.register_autograd("quartet_b200::rotary_qkv", _rotary_qkv_backward
 def fp8_linear_fwd(x: Tensor, w: Tensor, grad_dtype: torch.dtype, out_dtype: torch.dtype, need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
     """y = Q(x) Q(w)^T and what its backward needs: codes and scales of x and w transposed, as one buffer."""
     y, saved = ops.fp8_linear_fwd(x.contiguous(), w.contiguous(), need_dx, need_dw, out_dtype)
-    return y.contiguous(), saved
+    if x.numel() == 0:
+        saved = _u8(x, _saved_bytes(0, *w.shape, need_dx, need_dw))  # nothing is read from it
+    return _packed_rows(y), saved
 
 
 def _pad256(n: int) -> int:
     return (n + 255) // 256 * 256
 
 
+def _saved_bytes(m: int, N: int, K: int, need_dx: bool, need_dw: bool) -> int:
+    mp, np_ = _pad128(m), _pad128(N)
+    return (_pad256(K * mp) + _pad256(_sf_bytes(K, mp)) if need_dw else 0) + (_pad256(K * np_) + _pad256(_sf_bytes(K, np_)) if need_dx else 0)
+
+
+def _packed_rows(t: Tensor) -> Tensor:
+    """t without the padding behind its rows, in the strides that the fake kernels state (also where one row or none is contiguous as it is)."""
+    return t if t.shape[-1] * t.element_size() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 @fp8_linear_fwd.register_fake
 def _(x, w, grad_dtype, out_dtype, need_dx, need_dw):
     N, K = w.shape
-    m = x.numel() // K
-    mp, np_ = _pad128(m), _pad128(N)
-    saved = (_pad256(K * mp) + _pad256(_sf_bytes(K, mp)) if need_dw else 0) + (_pad256(K * np_) + _pad256(_sf_bytes(K, np_)) if need_dx else 0)
-    return x.new_empty((*x.shape[:-1], N), dtype=out_dtype), _u8(x, saved)
+    return x.new_empty((*x.shape[:-1], N), dtype=out_dtype), _u8(x, _saved_bytes(x.numel() // K, N, K, need_dx, need_dw))
 
 
 @torch.library.custom_op("quartet_b200::fp8_linear_bwd", mutates_args=())
@@ -578,7 +587,7 @@ def fp8_linear_bwd(e: Tensor, saved: Tensor, K: int, grad_dtype: torch.dtype, x_
         e2 = e2.float()
     dx, dw = ops.fp8_linear_bwd(e2 if e2.is_contiguous() else e2.contiguous(), saved, K, grad_dtype, x_dtype, w_dtype, need_dx, need_dw, need_dx, need_dw)
     ops.raise_on_fault("8-bit linear backward")  # only with QUARTET_CHECK_FAULTS=1
-    return (dx.contiguous() if need_dx else e.new_empty((0,), dtype=x_dtype)), (dw.contiguous() if need_dw else e.new_empty((0,), dtype=w_dtype))
+    return (_packed_rows(dx) if need_dx else e.new_empty((0,), dtype=x_dtype)), (_packed_rows(dw) if need_dw else e.new_empty((0,), dtype=w_dtype))
 
 
 @fp8_linear_bwd.register_fake

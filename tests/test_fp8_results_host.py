@@ -65,3 +65,24 @@ def test_operands_that_do_not_belong_together_are_refused(monkeypatch):
         with pytest.raises(ValueError):
             back(**bad)
     assert back(e=torch.zeros(0, 64), s=torch.empty(0, dtype=torch.uint8))[1].shape == (64, 256)
+
+
+@pytest.mark.parametrize("shape", [(0, 256), (3, 0, 256), (1, 256), (3, 5, 256), (300, 256)])
+@pytest.mark.parametrize("need", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("n", [64, 77])
+def test_operators_keep_the_shapes_they_state(shape, need, n):
+    """What the compiler is told of the layer's operators is what they return, without tokens too."""
+    from torch._subclasses import FakeTensorMode
+
+    x, w = torch.randn(shape), torch.randn(n, 256)
+    fwd, bwd = torch.ops.quartet_b200.fp8_linear_fwd, torch.ops.quartet_b200.fp8_linear_bwd
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    real = fwd(x, w, f8, f32, *need)
+    e = torch.zeros(*shape[:-1], n)
+    back = bwd(e, real[1], 256, f8, f32, f32, *need)
+    with FakeTensorMode() as mode:
+        fx, fw, fe = (mode.from_tensor(t) for t in (x, w, e))
+        told = fwd(fx, fw, f8, f32, *need)
+        told_back = bwd(fe, told[1], 256, f8, f32, f32, *need)
+    for a, b in zip((*real, *back), (*told, *told_back)):
+        assert a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype

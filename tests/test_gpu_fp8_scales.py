@@ -104,3 +104,22 @@ def test_results_changed_in_place_before_the_backward(ops, n):
         y.square().sum().backward()
         grads.append((y.detach(), a.grad, b.grad))
     assert all(torch.equal(u, v) for u, v in zip(*grads))
+
+
+@pytest.mark.parametrize("n", [64, 77])
+def test_compiled_layer_with_few_tokens_or_none(ops, n):
+    from quartet_b200.quantization import Fp8Linear
+
+    torch.manual_seed(0)
+    lin = Fp8Linear(200, n).cuda()
+    comp = torch.compile(lin, fullgraph=True, dynamic=False)
+    for tokens in (0, 1, 5):
+        grads = []
+        for f in (lin, comp):
+            x = torch.randn(2, tokens, 200, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).requires_grad_()
+            lin.weight.grad = None
+            y = f(x)
+            y.square().sum().backward()
+            grads.append((y.detach(), x.grad, lin.weight.grad.clone()))
+        assert grads[0][0].shape == (2, tokens, n)
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
