@@ -79,6 +79,11 @@ def forward_mode() -> bool:
     return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
+def recording() -> bool:
+    """Whether the call is being put into a graph (compiled, exported, traced), where only registered operators are seen."""
+    return (torch.compiler.is_compiling() or torch.jit.is_tracing()) and not forward_mode()
+
+
 def eagerly(fn, *args):
     """fn(*args) outside any graph being compiled: a compiler calls an autograd function's forward without its forward-mode derivative."""
     # (disable() loads the compiler, some four seconds, so it is called here and not as a decorator)
@@ -530,18 +535,24 @@ def linear_fp8(x, w, w_sf, out_dtype=None):
     if (x.requires_grad and torch.is_grad_enabled()) or has_tangent(x):
         raise RuntimeError("linear_fp8 has no derivative: call it under torch.no_grad() or on x.detach(), or use quantization.fp8_linear")
     _need_codes(w, w_sf, "linear_fp8")
-    shape, dev = x.shape, w.device
-    if len(shape) < 1 or shape[-1] < 1:
+    if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have at least one column")
-    K, N = shape[-1], w.shape[0]
-    if (K + 127) // 128 * 128 != w.shape[1]:
-        raise ValueError(f"x has {K} columns, the weight {w.shape[1]}")
-    if x.device != dev:
+    if (x.shape[-1] + 127) // 128 * 128 != w.shape[1]:
+        raise ValueError(f"x has {x.shape[-1]} columns, the weight {w.shape[1]}")
+    if x.device != w.device:
         raise ValueError("x and the weight are on different devices")
+    dtype = out_dtype or x.dtype
+    if recording():
+        return torch.ops.quartet_b200.linear_fp8(x, w, w_sf, dtype)
+    return _linear_fp8(x, w, w_sf, dtype)
+
+
+def _linear_fp8(x, w, w_sf, dtype):
+    shape, dev, N = x.shape, w.device, w.shape[0]
     if not x.is_contiguous():
         x = x.contiguous()
+    K = shape[-1]
     M = x.numel() // K
-    dtype = out_dtype or x.dtype
     xd, wd, yd = _dt(x), _f8(w.dtype), _out_dt(dtype)
     y, pitch = _padded_out(shape[:-1], N, dtype, dev)
     if M and N:

@@ -57,7 +57,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, grad_dtype: torch.dtype
         raise ValueError("x and weight must live on one CUDA device")
     ops._f8(grad_dtype)
     out_dtype = out_dtype or _out_dtype(x, x.dtype)
-    if (torch.compiler.is_compiling() or torch.jit.is_tracing()) and not ops.forward_mode():
+    if ops.recording():
         # a compiled graph is guarded on what needs a gradient; a trace is not, and may be called with other inputs, so it keeps both transposes
         need_dx, need_dw = (True, True) if torch.jit.is_tracing() else [torch.is_grad_enabled() and t.requires_grad for t in (x, weight)]
         return torch.ops.quartet_b200.fp8_linear_fwd(x, weight, grad_dtype, out_dtype, need_dx, need_dw)[0]

@@ -119,11 +119,6 @@ def _turn_by_mode(q, k, *args):
     return _Rotary.apply(q, None, *args)[0], _Rotary.apply(k, None, *args)[0]
 
 
-def _recording() -> bool:
-    """Whether the call is being put into a graph (compiled, exported, traced), where only registered operators are seen."""
-    return (torch.compiler.is_compiling() or torch.jit.is_tracing()) and not ops.forward_mode()
-
-
 def _check_heads(x, what):
     if x.dim() != 4:
         raise ValueError(f"{what} must be [batch, tokens, heads, d]")
@@ -135,7 +130,7 @@ def apply_rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=True, 
     _check_heads(q, "q")
     if k is not None:
         _check_heads(k, "k")
-    if _recording():
+    if ops.recording():
         turn = torch.ops.quartet_b200.rotary
         return (turn(q, inv_freq, positions, offset, interleaved, scale, False),
                 None if k is None else turn(k, inv_freq, positions, offset, interleaved, scale, False))
@@ -173,7 +168,7 @@ def rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions=None, *, offset=0, in
     (head_major, what scaled_dot_product_attention takes) or [batch, tokens, heads, d], each contiguous."""
     if qkv.dim() != 3 or n_head < 1 or n_kv_head < 1 or qkv.shape[2] % (n_head + 2 * n_kv_head) or qkv.shape[2] == 0:
         raise ValueError("qkv must be [batch, tokens, (n_head + 2 n_kv_head) * d]")
-    if _recording():
+    if ops.recording():
         return torch.ops.quartet_b200.rotary_qkv(qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)
     if ops.forward_mode():
         return ops.eagerly(_RotaryQKV.apply, qkv, n_head, n_kv_head, inv_freq, positions, offset, interleaved, scale, head_major)

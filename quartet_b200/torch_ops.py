@@ -613,3 +613,14 @@ def _fp8_linear_backward(ctx, e, *unused):
 
 
 torch.library.register_autograd("quartet_b200::fp8_linear_fwd", _fp8_linear_backward, setup_context=_fp8_linear_setup)
+
+
+@torch.library.custom_op("quartet_b200::linear_fp8", mutates_args=())
+def linear_fp8(x: Tensor, w: Tensor, w_sf: Tensor, out_dtype: torch.dtype) -> Tensor:
+    """x [..., K] times a packed weight (ops.linear_fp8)."""
+    return _packed_rows(ops._linear_fp8(x, w, w_sf, out_dtype))
+
+
+@linear_fp8.register_fake
+def _(x, w, w_sf, out_dtype):
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=out_dtype)

@@ -166,3 +166,16 @@ def test_the_packed_form_refuses_what_it_cannot_differentiate():
         ops.linear_fp8(fwad.make_dual(x, x), w, sf)
     with torch.no_grad(), pytest.raises(ValueError):            # a leaf of a model that is served: only the device is wrong here
         ops.linear_fp8(x.clone().requires_grad_(), w, sf)
+
+
+def test_the_packed_form_is_compiled_and_traced_as_one_operator(monkeypatch):
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_linear_fp8", lambda a, b, c, dt: _opaque(torch.nn.functional.pad(a.detach(), (0, 56)), b.float(), dt))
+    w, sf = torch.randn(8, 256).to(torch.float8_e4m3fn), torch.zeros(ops.sf_bytes(8, 256), dtype=torch.uint8)
+    x, z = torch.randn(2, 3, 200), torch.randn(2, 3, 200)
+    f = lambda a: ops.linear_fp8(a, w, sf) * 2  # noqa: E731
+    want = f(x)
+    assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(x), want) and want.shape == (2, 3, 8)
+    assert torch.equal(torch.jit.trace(f, (x,))(z), f(z))
+    with pytest.raises(Exception, match="no derivative"):
+        torch.compile(f, fullgraph=True, backend="aot_eager")(x.clone().requires_grad_())

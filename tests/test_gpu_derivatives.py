@@ -52,3 +52,18 @@ def test_traced_calls_compute():
                 assert torch.equal(a, b) and a.requires_grad == grad
                 if grad:
                     assert torch.equal(*(torch.autograd.grad(v.float().sum(), (z,), retain_graph=True)[0] for v in (a, b)))
+
+
+@pytest.mark.parametrize("m", [1, 40])
+@pytest.mark.parametrize("n", [64, 77])
+def test_the_packed_form_compiled_and_traced(m, n):
+    from quartet_b200 import ops
+
+    w, sf = ops.quant_fp8(torch.randn(n, 200, device="cuda"), square=True)[:2]
+    f = lambda a: ops.linear_fp8(a, w, sf, torch.bfloat16) * 2  # noqa: E731
+    x, z = torch.randn(m, 1, 200, device="cuda"), torch.randn(m, 1, 200, device="cuda")
+    assert torch.equal(torch.compile(f, fullgraph=True)(x), f(x))
+    assert torch.equal(torch.jit.trace(f, (x,))(z), f(z))
+    # calls that are no operators break a compiled graph, and compute what they do outside one
+    g = lambda a: ops.dequant_fp8(*ops.quant_fp8(a.view(m, 200))[:2], 200) * 2  # noqa: E731
+    assert torch.equal(torch.compile(g)(x), g(x))
