@@ -259,6 +259,18 @@ int quartet_dequant_fp8(const uint8_t* codes, const uint8_t* sf, int64_t rows, i
  */
 int quartet_gemm_fp8_tn(const uint8_t* a, const uint8_t* a_sf, int a_fmt, const uint8_t* b, const uint8_t* b_sf, int b_fmt, int64_t M, int64_t N, int64_t K,
                         float alpha, void* d, int d_dtype, int64_t ldd, quartet_stream_t stream);
+/*
+ * Which of its forms a product of these extents takes on the current device, and over how many CTAs of a cluster it splits the contraction.
+ */
+enum {
+    QUARTET_FP8_STREAM = 0,       /* up to eight rows of A: a stream over B */
+    QUARTET_FP8_PAIRS = 1,        /* CTA pairs, 256 x 256 results */
+    QUARTET_FP8_ROWS_256 = 2,     /* 256 rows of A and 128 of B a CTA */
+    QUARTET_FP8_ROWS_128 = 3,     /* 128 and 128, one CTA on an SM */
+    QUARTET_FP8_ROWS_128_TWO = 4, /* the same, two CTAs on an SM */
+    QUARTET_FP8_ROWS_FEW = 5      /* 32 or 64 rows of A, two CTAs on an SM */
+};
+int quartet_gemm_fp8_form(int64_t M, int64_t N, int64_t K, int32_t* form, int32_t* splits);
 
 /*
  * x [M, K] (bf16 / fp32) through a packed weight, y = alpha * Q(x) . W^T with Q the 1 x 128 quantizer above in e4m3: both steps in one call; up to

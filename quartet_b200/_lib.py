@@ -47,6 +47,7 @@ SIGNATURES = {
     "quartet_quant_fp8": (_i, [_p, _i, _i64, _i64, _i, _i, _p, _p, _p, _p, _p]),
     "quartet_dequant_fp8": (_i, [_p, _p, _i64, _i64, _i, _f, _p, _i, _p]),
     "quartet_gemm_fp8_tn": (_i, [_p, _p, _i, _p, _p, _i, _i64, _i64, _i64, _f, _p, _i, _i64, _p]),
+    "quartet_gemm_fp8_form": (_i, [_i64, _i64, _i64, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "quartet_linear_fp8_workspace_bytes": (_i64, [_i64, _i64]),
     "quartet_linear_fp8": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i64, _f, _p, _p, _i, _i64, _p]),
     "quartet_linear_fp8_train_bytes": (_i, [_i64, _i64, _i64, _i, _i, _p]),

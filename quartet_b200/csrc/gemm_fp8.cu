@@ -742,7 +742,14 @@ static int resident_clusters(const int (**out)[4]) {
 constexpr struct { int chunk, start, again; } COST_PAIR{6, 115, 35};
 constexpr struct { int chunk, start, join; } COST_256{6, 140, 30}, COST_128{5, 105, 30}, COST_128_TWO{5, 150, 30}, COST_FEW{5, 150, 8};
 
-enum class Way { FEW_TOKENS, PAIR, ROWS_256, ROWS_128, ROWS_128_TWO, ROWS_FEW };
+enum class Way {
+    FEW_TOKENS = QUARTET_FP8_STREAM,
+    PAIR = QUARTET_FP8_PAIRS,
+    ROWS_256 = QUARTET_FP8_ROWS_256,
+    ROWS_128 = QUARTET_FP8_ROWS_128,
+    ROWS_128_TWO = QUARTET_FP8_ROWS_128_TWO,
+    ROWS_FEW = QUARTET_FP8_ROWS_FEW
+};
 
 static int pick_way(const Fp8GemmParams& p, Way* way, int* splits, int64_t* cost) {
     *way = Way::FEW_TOKENS, *splits = 1, *cost = 0;
@@ -825,9 +832,30 @@ int product_two(const Fp8Product& x, const Fp8Product& y, cudaStream_t s) {
     return rc ? rc : run_way(y, wy, sy, s);
 }
 
+static int check_extents(int64_t M, int64_t N, int64_t K) {
+    if (M < 1 || N < 1 || K < 128 || K % 128 || M > 8388480 || N > 8388480 || K > (1 << 30))
+        return fail(QUARTET_E_SHAPE, "need 1 <= M, N <= 8388480 and K a multiple of 128 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
+    return QUARTET_OK;
+}
+
 }  // namespace quartet
 
 using namespace quartet;
+
+extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_form(int64_t M, int64_t N, int64_t K, int32_t* form, int32_t* splits) {
+    if (!form || !splits) return fail(QUARTET_E_NULL, "form and splits must be non-NULL");
+    int rc = check_extents(M, N, K);
+    if (rc) return rc;
+    if ((rc = check_device())) return rc;
+    Fp8GemmParams p{};
+    p.M = M, p.N = N, p.k_chunks = (int)(K / 128);
+    Way way;
+    int64_t cost;
+    int s = 1;
+    if ((rc = pick_way(p, &way, &s, &cost))) return rc;
+    *form = (int32_t)way, *splits = s;
+    return QUARTET_OK;
+}
 
 extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_tn(const uint8_t* a, const uint8_t* a_sf, int a_fmt, const uint8_t* b,
                                                                           const uint8_t* b_sf, int b_fmt, int64_t M, int64_t N, int64_t K, float alpha,
@@ -836,12 +864,11 @@ extern "C" __attribute__((visibility("default"))) int quartet_gemm_fp8_tn(const 
     if ((a_fmt != QUARTET_E4M3 && a_fmt != QUARTET_E5M2) || (b_fmt != QUARTET_E4M3 && b_fmt != QUARTET_E5M2))
         return fail(QUARTET_E_ARG, "a_fmt and b_fmt must be 0 (e4m3) or 1 (e5m2)");
     if (d_dtype != QUARTET_BF16 && d_dtype != QUARTET_F32) return fail(QUARTET_E_ARG, "d_dtype must be 0 or 1");
-    if (M < 1 || N < 1 || K < 128 || K % 128 || M > 8388480 || N > 8388480 || K > (1 << 30))
-        return fail(QUARTET_E_SHAPE, "need 1 <= M, N <= 8388480 and K a multiple of 128 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
+    int rc = check_extents(M, N, K);
+    if (rc) return rc;
     if (ldd < N || ldd % (d_dtype == QUARTET_F32 ? 4 : 8)) return fail(QUARTET_E_SHAPE, "rows of d must start on 16-byte boundaries and hold N results");
     if (!aligned16(a) || !aligned16(b) || !aligned16(a_sf) || !aligned16(b_sf) || !aligned16(d)) return fail(QUARTET_E_ALIGN, "operands must be 16-byte aligned");
-    int rc = bind_context_of(a);
-    if (rc) return rc;
+    if ((rc = bind_context_of(a))) return rc;
     if ((rc = check_device())) return rc;
     Fp8GemmParams p{};
     p.a_sf = a_sf, p.b_sf = b_sf;

@@ -528,6 +528,16 @@ def gemm_fp8_tn(a, a_sf, b, b_sf, alpha=1.0, out_dtype=torch.bfloat16):
     return out
 
 
+GEMM_FP8_FORMS = ("stream", "pairs", "rows_256", "rows_128", "rows_128_two", "rows_few")
+
+
+def gemm_fp8_form(M, N, K):
+    """(form, ways the contraction is split) of a product of these extents (K a multiple of 128) on the current device."""
+    form, splits = C.c_int32(0), C.c_int32(0)
+    _lib.check(_lib.load().quartet_gemm_fp8_form(M, N, K, C.byref(form), C.byref(splits)), "quartet_gemm_fp8_form")
+    return GEMM_FP8_FORMS[form.value], splits.value
+
+
 def linear_fp8(x, w, w_sf, out_dtype=None):
     """x [..., K] times a packed weight (codes [N, pad128(K)] and scales of quant_fp8(weight, square=True)) -> [..., N]: x is quantized in
     blocks of 128 (e4m3) and multiplied.  The serving form of quantization.fp8_linear; not differentiable: an x that wants a gradient, or has a
