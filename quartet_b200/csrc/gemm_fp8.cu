@@ -313,8 +313,7 @@ struct PairCfg {
     static constexpr int B_BYTES = 128 * 128;                // this CTA's half of B's rows
     static constexpr int SFA_BYTES = 512, SFB_BYTES = 1024;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int NBUF = 1;                           // staging buffers of an epilogue warp, 4 KB each
-    static constexpr int STG_BYTES = 8 * NBUF * 4096;
+    static constexpr int STG_BYTES = 8 * 4096;               // a staging buffer for each epilogue warp
     static constexpr int STAGES = (232448 - STG_BYTES - 512) / STAGE_BYTES;
     static constexpr int SMEM = STAGES * STAGE_BYTES + STG_BYTES + 512;
     // Consecutive tiles accumulate in columns [0, 256) and [128, 384): the 128 they share are drained into registers first, so
@@ -339,9 +338,8 @@ __device__ __forceinline__ void tc_mma2_mxf8(uint32_t d_tmem, uint64_t adesc, ui
 // 32 rows x 64 columns of results, one row per thread, through 4 KB of swizzled staging to global memory: one tensor store of 64 bf16
 // columns or two of 32 fp32 columns, 128 bytes a row.  A tensor store clips only to whole 16-byte units of a row (measured: the rest of the last
 // unit is written as zeros), so the tensor map ends with the last whole unit, at n_whole, and the few columns behind it are written value by value.
-template <int NBUF>
 __device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const uint32_t (&r1)[32], const Fp8GemmParams& p, const CUtensorMap* tm_d, int row0,
-                                              int col, uint8_t* stg, uint32_t& n_stores, int lane) {
+                                              int col, uint8_t* stg, int lane) {
     const int n_whole = (int)p.N & (p.d_f32 ? ~3 : ~7);
     if (n_whole < p.N && col + 64 > n_whole) {
         const int64_t row = (int64_t)row0 + lane;
@@ -358,18 +356,15 @@ __device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const ui
         }
     }
     if (col >= n_whole) return;
-    auto slot = [&]() -> uint8_t* {
-        uint8_t* buf = stg + (n_stores % NBUF) * 4096;
-        ++n_stores;
-        if (lane == 0) { if (NBUF == 2) bulk_wait_read1(); else bulk_wait_read0(); }
+    auto staging_free = [&]() {  // the store before has been read from it
+        if (lane == 0) bulk_wait_read0();
         __syncwarp();
-        return buf;
     };
-    auto send = [&](uint8_t* buf, int c) {
+    auto send = [&](int c) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-            tma_store_2d(tm_d, c, row0, buf);
+            tma_store_2d(tm_d, c, row0, stg);
             bulk_commit();
         }
     };
@@ -377,18 +372,18 @@ __device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const ui
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (col + 32 * h >= n_whole) break;
-            uint8_t* buf = slot();
+            staging_free();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float v[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(h ? r1[4 * j + k] : r0[4 * j + k]) * p.alpha;
-                *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
             }
-            send(buf, col + 32 * h);
+            send(col + 32 * h);
         }
     } else {
-        uint8_t* buf = slot();
+        staging_free();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             uint32_t w[4];
@@ -398,9 +393,9 @@ __device__ __forceinline__ void store_block64(const uint32_t (&r0)[32], const ui
                 const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(j < 4 ? r0[i] : r1[i]) * p.alpha, __uint_as_float(j < 4 ? r0[i + 1] : r1[i + 1]) * p.alpha);
                 w[k] = *reinterpret_cast<const uint32_t*>(&t);
             }
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        send(buf, col);
+        send(col);
     }
 }
 
@@ -607,8 +602,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else {
         // two warps per lane quadrant; each takes one 64-column block of the shared half of the accumulator, then one of the other half
         const int q = warp & 3, par = warp >= 11 ? 1 : 0;
-        uint8_t* stg = s_stg + (par * 4 + q) * (C::NBUF * 4096);
-        uint32_t acc_it = 0, n_stores = 0;
+        uint8_t* stg = s_stg + (par * 4 + q) * 4096;
+        uint32_t acc_it = 0;
         for (; !*dead && tiles.next(product, tile); ++acc_it) {
             const Fp8GemmParams& p = second() ? p1.g : p0;
             const CUtensorMap* d_map = second() ? &p1.tm.d : &tm_d;
@@ -628,11 +623,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(acc_empty), 0));
             const bool rows = row0 < p.M;
-            if (rows && n0 + c0 < p.N) store_block64<C::NBUF>(r0, r1, p, d_map, row0, n0 + c0, stg, n_stores, lane);
+            if (rows && n0 + c0 < p.N) store_block64(r0, r1, p, d_map, row0, n0 + c0, stg, lane);
             tc_ld32(t0 + c1, r0);
             tc_ld32(t0 + c1 + 32, r1);
             tc_wait_ld();
-            if (rows && n0 + c1 < p.N) store_block64<C::NBUF>(r0, r1, p, d_map, row0, n0 + c1, stg, n_stores, lane);
+            if (rows && n0 + c1 < p.N) store_block64(r0, r1, p, d_map, row0, n0 + c1, stg, lane);
             tc_fence_before();  // all of this tile's tensor-memory reads are complete before the warp's next arrive
         }
         if (lane == 0) bulk_wait0();

@@ -118,12 +118,7 @@ __device__ __forceinline__ void tmem_relinquish2() {
 __device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// arrive on a barrier (given by its shared::cluster address) once all MMAs issued so far are done
-__device__ __forceinline__ void tc_commit2(uint32_t cluster_addr) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr)
-                 : "memory");
-}
-// the same, arriving on the barrier at this shared-memory offset in BOTH CTAs of the pair (one
+// arrive, once all MMAs issued so far are done, on the barrier at this shared-memory offset in BOTH CTAs of the pair (one
 // instruction instead of two commits; only the completion signal is multicast, no data copy)
 __device__ __forceinline__ void tc_commit2_pair(uint32_t own_addr) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
