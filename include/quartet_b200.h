@@ -311,8 +311,8 @@ int quartet_rotary(int n_seg, const void* const* src, void* const* dst, const in
 
 /*
  * Norm over n tensors (clip_grad_norm_ of src/optim/base.py:203-204) and clipping by it, in two launches for any number of tensors up to 768.
- * grads, numels, dtypes (bf16 / fp32, mixed) are HOST arrays.  kind 0: square root of the sum of squares, taken and added in 64 bits;
- * kind 1: largest magnitude.  workspace: QUARTET_NORM_PARTIALS doubles of device memory.
+ * grads, numels, dtypes (bf16 / fp32, mixed) are HOST arrays.  kind 0: square root of the sum of squares, taken and added in 64 bits (four
+ * squares of bf16 values, each exact in 32 bits, may be joined there first: 2^-24 of the norm at most); kind 1: largest magnitude.  workspace: QUARTET_NORM_PARTIALS doubles of device memory.
  * quartet_grad_norm: *total = sum of squares (kind 1: the maximum), what ranks that hold different tensors add up (take the largest of);
  * *norm the norm in fp32.  Either may be NULL.
  * quartet_clip_grads: outs[i] = grads[i] * c, c = min(1, max_norm / (norm + 1e-6)), NaN where the norm is NaN; outs[i] may be grads[i]; otherwise no

@@ -724,7 +724,7 @@ static int resident_clusters(const int (**out)[4]) {
     return QUARTET_OK;
 }
 
-// Which kernel, and how many ways the contraction is split.  Up to eight rows: the stream over B.  Else the way that takes the least by a model in
+// Which kernel, and how many ways the contraction is split.  Up to eight rows: the stream over B (both sides' times are in gemv_fp8.cu).  Else the way that takes the least by a model in
 // units of 40 ns: a round of resident tiles takes `chunk` for every 128 values of its part of the contraction and `start` for its beginning and end, of
 // which a persistent kernel pays `again` in its later rounds, and a cluster that adds partial results takes `join` more.
 // Over 84 shapes (M 9 to 32000, N 100 to 32000, K 128 to 32000) the way taken is 2 % behind the best one on average, 19 % at most.

@@ -7,12 +7,21 @@
 // block: no tensor memory, no cluster.  All SMs take part evenly, which the memory's rate needs: one SM draws at most about 24 bytes a clock from
 // it, however many copies are under way.
 // The products are m16n8k16 in fp16, which holds every 8-bit code: 16 rows of B, converted as they come from shared memory, and the
-// (up to) eight rows of A, converted once.  Sums over 32 values are scaled by their two E8M0 factors in fp32 and added to
-// fp32 sums, which the warps of a group join in a fixed order in shared memory.  (The 8-bit form of the instruction converts both operands
-// inside: 30 us at N 12288, K 4096, one row, where this takes 14.)  Bound by the issue of instructions before the memory: eight warps instead of
-// sixteen took half as long again, and 32 warps or deeper rings gain nothing.
-// us at one row, quantizer included, here / tensor-memory kernel behind its quantizer: N 12288, K 4096 14.1 / 15.5; N 4096, K 11008 12.6 / 13.7;
-// N 32000, K 640 7.1 / 7.7.
+// (up to) eight rows of A, converted once.  Sums over the 128 values of a chunk (over 32, where the scales differ inside it) are scaled in fp32 and
+// added to fp32 sums, which the warps of a group join in a fixed order in shared memory.  (The 8-bit form of the instruction converts both
+// operands inside: 30 us at N 12288, K 4096, one row, where this takes 14.)
+// Bound by the latency of a warp's chain from a chunk's copy over its conversions and products to the sum, which four warps a scheduler cover in
+// part: at N 12288, K 4096 and one row 6.8 M warp instructions fill 49 % of the issue slots and the memory is 36 % busy, 4 us of the launch
+// among them.  Eight warps instead of sixteen took half as long again; 32 warps or deeper rings gain nothing.
+// us, quantizer included, weights from memory, 1 / 4 / 8 rows here | tensor-memory kernel behind its quantizer:
+//     N  1920, K   640     3.9   4.1   4.2  |   5.2   5.4   5.6
+//     N  4096, K  4096     6.9   7.2   8.5  |   8.4   8.6   8.7
+//     N 32000, K   640     7.5   8.0   8.5  |   7.9   7.9   8.1
+//     N  4096, K 11008    12.1  14.4  13.7  |  13.2  13.4  13.6
+//     N 12288, K  4096    13.8  14.1  15.4  |  13.9  14.2  13.7
+//     N 32000, K  4096    27.7  28.5  30.3  |  24.8  24.9  25.1
+// So eight rows as the limit whatever the size gains up to a quarter on small weights and loses a tenth to a fifth on the largest.  It stays a rule
+// on M and K alone because it also decides whether a call needs a workspace, whose size is asked for without N.
 // A comes as codes and scales, or as values that the CTA quantizes into shared memory while its first copies are under way.
 #include "common.cuh"
 #include "gemm_fp8.cuh"
@@ -65,7 +74,7 @@ struct GemvParams {
     int64_t a_cols;         // values in a row (A_BF16, A_F32)
     int a_vec;
     int kw;                 // warps that share a row group's contraction
-    int blocks;             // blocks of 16 * 8 / kw rows
+    int blocks;             // blocks of 16 * GEMV_WARPS / kw rows
 };
 
 template <int AMODE, bool B_E5M2, bool A_E5M2>
