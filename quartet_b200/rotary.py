@@ -37,8 +37,12 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
     if scaling is not None:
         opts = dict(scaling)
         kind, f = opts.pop("kind", None), float(opts.pop("factor", 1.0))
-        if f < 1.0:
-            raise ValueError("factor must be at least 1")
+        if not 1.0 <= f < math.inf:
+            raise ValueError("factor must be finite and at least 1")
+        if kind in ("bands", "yarn"):
+            length = float(opts.pop("original_length", 0.0))
+            if not length > 0:
+                raise ValueError(f"{kind} scaling needs an original_length above 0")
         if kind == "linear":
             inv = inv / f
         elif kind == "ntk":
@@ -46,14 +50,17 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
                 raise ValueError("ntk scaling needs at least two pairs")
             inv = (base * f ** (rot_dim / (rot_dim - 2))) ** -exponent
         elif kind == "bands":
-            length, low, high = float(opts.pop("original_length")), float(opts.pop("low", 1.0)), float(opts.pop("high", 4.0))
+            low, high = float(opts.pop("low", 1.0)), float(opts.pop("high", 4.0))
             if not 0 < low < high:
                 raise ValueError("need 0 < low < high")
             keep = ((length * inv / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
             inv = (1.0 - keep) * inv / f + keep * inv
         elif kind == "yarn":
-            length = float(opts.pop("original_length"))
             fast, slow = float(opts.pop("beta_fast", 32.0)), float(opts.pop("beta_slow", 1.0))
+            if not 0 < slow <= fast:
+                raise ValueError("need 0 < beta_slow <= beta_fast")
+            if base == 1.0:
+                raise ValueError("yarn scaling needs a base other than 1")
 
             def pair(turns):
                 return rot_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
