@@ -457,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     uint64_t* empty = full + C::STAGES;          // local: the pair's MMAs are done with the stage
     uint64_t* sf_full = empty + C::STAGES;       // leader: 8 feeder warps (both CTAs) have fed the stage
     uint64_t* sf_land = sf_full + C::STAGES;     // local: the stage's scale blocks have landed
-    uint64_t* sf_free = sf_land + C::STAGES;     // local: the 4 feeder warps hold the stage's scales in registers
+    uint64_t* sf_free = sf_land + C::STAGES;     // local: the 4 feeder warps have the stage's scales in tensor memory
     uint64_t* acc_full = sf_free + C::STAGES;    // local: accumulator complete
     uint64_t* acc_empty = acc_full + 1;          // leader: 16 epilogue warps (both CTAs) have drained the shared columns
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_empty + 1);
@@ -583,8 +583,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 const uint4 v0 = *reinterpret_cast<const uint4*>(s_sfb + s * C::SFB_BYTES + lane * 16);
                 const uint4 v1 = *reinterpret_cast<const uint4*>(s_sfb + s * C::SFB_BYTES + 512 + lane * 16);
                 const uint32_t ra[8] = {va.x, va.y, va.z, va.w, 0, 0, 0, 0}, rb[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_free[s]);
                 if (it >= (uint32_t)C::SF_SLOTS) {
                     const uint32_t pit = it - C::SF_SLOTS;
                     if (!gemm_wait(&empty[pit % C::STAGES], (pit / C::STAGES) & 1, WAIT_GEMM_EMPTY, dead)) break;
@@ -594,6 +592,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 tc_st8(sf + 4, rb);
                 tc_wait_st();
                 tc_fence_before();
+                __syncwarp();
+                // Only now is the buffer given back, when the scales have left it for certain.  An arrive behind the loads alone let the copy of five
+                // chunks later overtake them where operands were late: scales of chunk c + 5 on chunk c in one of some 200 products from cold memory.
+                if (lane == 0) mbar_arrive(&sf_free[s]);
                 if (!gemm_wait(&full[s], ph, WAIT_GEMM_FULL, dead)) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&sf_full[s]), 0));
