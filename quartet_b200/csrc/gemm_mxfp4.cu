@@ -448,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM2_THREADS, 1)
     uint64_t* empty = full + C::STAGES;               // local: the pair's MMAs are done with the stage
     uint64_t* sf_full = empty + C::STAGES;            // leader only: 8 feeder warps (both CTAs) have fed the stage
     uint64_t* sf_land = sf_full + C::STAGES;          // local: the stage's scale blocks have landed
-    uint64_t* sf_free = sf_land + C::STAGES;          // local: the 4 feeder warps hold the stage's scales in registers
+    uint64_t* sf_free = sf_land + C::STAGES;          // local: the 4 feeder warps have the stage's scales in tensor memory
     uint64_t* acc_full = sf_free + C::STAGES;         // local: accumulator complete
     uint64_t* acc_empty = acc_full + C::ACC_STAGES;   // leader only: 8 epilogue warps (both CTAs) have drained it
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_empty + C::ACC_STAGES);
@@ -513,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM2_THREADS, 1)
                 const uint8_t* sfa_src = p.a_sf + (int64_t)m_blk * sf_blocks_per_rowblock * 512;
                 for (int ks = 0; ks < k_stages; ++ks) {
                     // operand buffers are free once the stage's MMAs are done; the scale buffers as soon as the
-                    // feeders have them in registers, so the scale copies run several stages ahead
+                    // feeders have them in tensor memory, so the scale copies run several stages ahead
                     if (!gemm_wait(role == 2 ? &sf_free[s] : &empty[s], ph ^ 1, WAIT_GEMM_EMPTY, dead)) break;
                     if (role == 0) {
                         mbar_arrive_expect_tx(&full[s], C::A_BYTES);
@@ -620,8 +620,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM2_THREADS, 1)
                                        : 0u;
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_free[s]);  // the scale copies of a later stage may reuse the buffers
                 // the scale slot was last read by the MMAs of iteration it - SF_SLOTS; their completion is
                 // what the `empty` barrier of that iteration's operand stage reports
                 if (it >= (uint32_t)C::SF_SLOTS) {
@@ -641,6 +639,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM2_THREADS, 1)
                 }
                 tc_wait_st();
                 tc_fence_before();
+                __syncwarp();
+                // The copies of a later stage may reuse the buffers only now, when the scales have left them for certain: an arrive behind the loads
+                // alone lets a copy overtake them (seen in the 8-bit kernel, which feeds its scales alike).
+                if (lane == 0) mbar_arrive(&sf_free[s]);
                 // the scales usually sit in tensor memory before the operands arrive; the arrive below tells
                 // the MMA issuer that BOTH are there for this CTA
                 if (!gemm_wait(&full[s], ph, WAIT_GEMM_FULL, dead)) break;
