@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, CTAS) gemm_fp8_split_kernel(con
             const uint4* sf = reinterpret_cast<const uint4*>(s_sf + s * C::SF_BYTES) + lane;
             const uint4 w4 = sf[0], x4 = sf[32];
             const uint32_t v[8] = {w4.x, w4.y, w4.z, w4.w, x4.x, x4.y, x4.z, x4.w};
+            __syncwarp();  // (a wait's lanes may leave it apart; tensor-memory instructions are the warp's)
             tc_st8(tmem + lane_base + C::SF_COL0 + s * C::SF_COLS, v);
             if constexpr (C::X_BLOCKS == 2) {
                 const uint4 z4 = sf[64];
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, CTAS) gemm_fp8_split_kernel(con
     }
     __syncwarp();
     // ---- partial results [token][weight row] in fp32 over the operand stages: all copies have landed and been read ----
-    const bool ok = gemm_wait(acc_full, 0, WAIT_GEMM_ACC_FULL, dead);
+    const bool ok = gemm_wait_warp(acc_full, 0, WAIT_GEMM_ACC_FULL, dead);
     tc_fence_after();
     float* red = reinterpret_cast<float*>(smem);
     const int row = (warp & 3) * 32 + lane;
@@ -588,6 +589,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     if (!gemm_wait(&empty[pit % C::STAGES], (pit / C::STAGES) & 1, WAIT_GEMM_EMPTY, dead)) break;
                     tc_fence_after();
                 }
+                __syncwarp();  // (a wait's lanes may leave it apart; tensor-memory instructions are the warp's)
                 tc_st4(sf, ra);
                 tc_st8(sf + 4, rb);
                 tc_wait_st();
@@ -612,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             coords();
             const int n0 = n_blk * C::BN;
             const int row0 = (m_pair * 2 + (int)rank) * 128 + q * 32;
-            if (!gemm_wait(acc_full, acc_it & 1, WAIT_GEMM_ACC_FULL, dead)) break;
+            if (!gemm_wait_warp(acc_full, acc_it & 1, WAIT_GEMM_ACC_FULL, dead)) break;
             tc_fence_after();
             const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (acc_it & 1) * C::ACC_SHIFT;
             const int first = (acc_it & 1) ? 0 : 128;         // the half that the next tile's accumulator overlaps

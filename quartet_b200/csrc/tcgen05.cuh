@@ -78,6 +78,13 @@ __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, int32_
     return false;
 }
 
+// The same for a whole warp: its lanes poll for themselves, so they may leave the wait apart, and one may give up as another sees the
+// barrier complete.  They go on together and with one answer, as warp-wide instructions (tcgen05.ld / st, elect.sync) and the warp's own
+// barriers need it.
+__device__ __forceinline__ bool gemm_wait_warp(uint64_t* bar, uint32_t parity, int32_t who, volatile int* dead) {
+    return __all_sync(0xFFFFFFFFu, gemm_wait(bar, parity, who, dead));
+}
+
 // One lane of a fully converged warp (elect.sync): the issuing warp runs its loop on all 32 lanes so
 // that ring indices, descriptors and addresses stay warp-uniform, and only the tcgen05 instructions
 // themselves are predicated on the elected lane.
