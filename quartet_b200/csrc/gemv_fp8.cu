@@ -14,13 +14,13 @@
 // part: at N 12288, K 4096 and one row 6.8 M warp instructions fill 49 % of the issue slots and the memory is 36 % busy, 4 us of the launch
 // among them.  Eight warps instead of sixteen took half as long again; 32 warps or deeper rings gain nothing.
 // us, quantizer included, weights from memory, 1 / 4 / 8 rows here | tensor-memory kernel behind its quantizer:
-//     N  1920, K   640     3.9   4.1   4.2  |   5.2   5.4   5.6
-//     N  4096, K  4096     6.9   7.2   8.5  |   8.4   8.6   8.7
-//     N 32000, K   640     7.5   8.0   8.5  |   7.9   7.9   8.1
-//     N  4096, K 11008    12.1  14.4  13.7  |  13.2  13.4  13.6
-//     N 12288, K  4096    13.8  14.1  15.4  |  13.9  14.2  13.7
-//     N 32000, K  4096    27.7  28.5  30.3  |  24.8  24.9  25.1
-// So eight rows as the limit whatever the size gains up to a quarter on small weights and loses a tenth to a fifth on the largest.  It stays a rule
+//     N  1920, K   640     3.8   4.0   4.1  |   5.2   5.4   5.6
+//     N  4096, K  4096     6.7   7.1   8.4  |   8.4   8.6   8.7
+//     N 32000, K   640     7.4   7.8   8.5  |   7.9   7.9   8.1
+//     N  4096, K 11008    11.8  14.1  13.6  |  13.2  13.4  13.6
+//     N 12288, K  4096    13.5  13.9  15.2  |  13.9  14.2  13.7
+//     N 32000, K  4096    26.4  27.3  29.0  |  24.8  24.9  25.1
+// So eight rows as the limit whatever the size gains up to a quarter on small weights and loses up to a sixth on the largest.  It stays a rule
 // on M and K alone because it also decides whether a call needs a workspace, whose size is asked for without N.
 // A comes as codes and scales, or as values that the CTA quantizes into shared memory while its first copies are under way.
 #include "common.cuh"
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
                     dead = true;
                     break;
                 }
+                __syncwarp();  // (the wait's lanes may leave it apart; ldmatrix and the products are the warp's)
                 --ahead;
                 const uint8_t* sfw = s_sf + s * GEMV_SF_BYTES + seg * 4 + g * 16;
                 const uint32_t w0 = *reinterpret_cast<const uint32_t*>(sfw), w1 = *reinterpret_cast<const uint32_t*>(sfw + 128);
@@ -216,14 +217,15 @@ __global__ void __launch_bounds__(GEMV_THREADS) gemv_fp8_kernel(const __grid_con
                     mma_f16_first(cc[k], f16x2_of<B_E5M2>(f[0]), f16x2_of<B_E5M2>(f[1]), f16x2_of<B_E5M2>(f[0] >> 16), f16x2_of<B_E5M2>(f[1] >> 16), xa.x, xa.y);
                     mma_f16(cc[k], f16x2_of<B_E5M2>(f[2]), f16x2_of<B_E5M2>(f[3]), f16x2_of<B_E5M2>(f[2] >> 16), f16x2_of<B_E5M2>(f[3] >> 16), xb.x, xb.y);
                 }
-                __syncwarp();
-                fill((int)s);  // the stage is in registers: its next copy may start
-                if (++s == GEMV_STAGES) s = 0, ph ^= 1;
                 // Two factors 2^(b - 127) make one, 2^(w + x - 254), taken as a whole: either by itself may lead out of fp32 where the product is well
                 // inside.  One scale for the whole chunk, as this library's quantizers write them, and bytes of 64 .. 190, whose sums leave a normal factor:
                 const bool block = w0 == __byte_perm(w0, 0, 0) && w1 == __byte_perm(w1, 0, 0) && x0 == __byte_perm(x0, 0, 0) && x1 == __byte_perm(x1, 0, 0);
                 constexpr uint32_t LOW = 64u << 24, SPAN = 127u << 24, ONE = 127u << 23;
-                if (__all_sync(0xFFFFFFFFu, block && max(max(w0 - LOW, w1 - LOW), max(x0 - LOW, x1 - LOW)) < SPAN)) {
+                const bool plain = __all_sync(0xFFFFFFFFu, block && max(max(w0 - LOW, w1 - LOW), max(x0 - LOW, x1 - LOW)) < SPAN);
+                __syncwarp();
+                fill((int)s);  // the stage has been read, its scales by the vote above: its next copy may start
+                if (++s == GEMV_STAGES) s = 0, ph ^= 1;
+                if (plain) {
                     const uint32_t f0 = (w0 >> 1) & 0x7F800000u, f1 = (w1 >> 1) & 0x7F800000u, g0 = (x0 >> 1) & 0x7F800000u, g1 = (x1 >> 1) & 0x7F800000u;
                     const float s00 = __uint_as_float(f0 + g0 - ONE), s01 = __uint_as_float(f0 + g1 - ONE);
                     const float s10 = __uint_as_float(f1 + g0 - ONE), s11 = __uint_as_float(f1 + g1 - ONE);
