@@ -85,9 +85,8 @@ def recording() -> bool:
 
 
 def eagerly(fn, *args):
-    """fn(*args) outside any graph being compiled: a compiler calls an autograd function's forward without its forward-mode derivative."""
-    # (disable() loads the compiler, some four seconds, so it is called here and not as a decorator)
-    return torch.compiler.disable(fn)(*args)
+    """fn(*args), outside the graph where one is being compiled: a compiler calls an autograd function's forward without its forward-mode derivative."""
+    return torch.compiler.disable(fn)(*args) if torch.compiler.is_compiling() else fn(*args)
 
 
 def has_tangent(*ts) -> bool:

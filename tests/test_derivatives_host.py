@@ -179,3 +179,22 @@ def test_the_packed_form_is_compiled_and_traced_as_one_operator(monkeypatch):
     assert torch.equal(torch.jit.trace(f, (x,))(z), f(z))
     with pytest.raises(Exception, match="no derivative"):
         torch.compile(f, fullgraph=True, backend="aot_eager")(x.clone().requires_grad_())
+
+
+def test_forward_mode_does_not_load_the_compiler():
+    """Loading it takes seconds; only a call inside compiled code needs it."""
+    import os
+    import subprocess
+    import sys
+
+    code = """if True:
+        import sys, torch
+        from torch.autograd import forward_ad as fwad
+        from quartet_b200 import ops, rotary
+        ops.rotary = lambda segments, *a: [dst.detach().copy_(src.detach()) for src, dst, _ in segments]
+        x = torch.randn(1, 2, 1, 8)
+        with fwad.dual_level():
+            y = rotary.apply_rotary(fwad.make_dual(x, x + 1), None, torch.ones(4, dtype=torch.float64))[0]
+            assert torch.equal(fwad.unpack_dual(y).tangent, x + 1)
+        sys.exit('torch._dynamo' in sys.modules)"""
+    assert subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__)))).returncode == 0
