@@ -253,13 +253,13 @@ static inline int64_t floor_div(int64_t a, int64_t b) {
 
 // 1: some choice of coefficients from axis i on adds up to `left` (`moved`: a choice of another address than a tensor's with itself), 0: none, -1: not
 // found in ROT_SEARCH steps.  lo, hi: what the axes from i on reach.
-static int rot_meets(const RotAxis* ax, int n, int i, int64_t left, int64_t lo, int64_t hi, bool moved, int& budget) {
+static int rot_meets(const RotAxis* ax, int n, int i, int64_t left, int64_t lo, int64_t hi, bool moved, int& steps) {
     if (i == n) return left == 0 && moved;
     lo -= ax[i].lo * ax[i].st, hi -= ax[i].hi * ax[i].st;
     const int64_t first = std::max(ax[i].lo, -floor_div(hi - left, ax[i].st)), last = std::min(ax[i].hi, floor_div(left - lo, ax[i].st));
     for (int64_t c = first; c <= last; ++c) {
-        if (--budget < 0) return -1;
-        const int r = rot_meets(ax, n, i + 1, left - c * ax[i].st, lo, hi, moved || c != 0, budget);
+        if (--steps < 0) return -1;
+        const int r = rot_meets(ax, n, i + 1, left - c * ax[i].st, lo, hi, moved || c != 0, steps);
         if (r) return r;
     }
     return 0;
@@ -268,8 +268,8 @@ static int rot_search(RotAxis* ax, int n, int64_t left, bool moved) {
     std::sort(ax, ax + n, [](const RotAxis& x, const RotAxis& y) { return x.st > y.st; });
     int64_t lo = 0, hi = 0;
     for (int k = 0; k < n; ++k) lo += ax[k].lo * ax[k].st, hi += ax[k].hi * ax[k].st;
-    int budget = ROT_SEARCH;
-    return rot_meets(ax, n, 0, left, lo, hi, moved, budget);
+    int steps = ROT_SEARCH;
+    return rot_meets(ax, n, 0, left, lo, hi, moved, steps);
 }
 // Whether two indexes of one tensor share an address.
 static int rot_folds(const RotSpan& a) {
