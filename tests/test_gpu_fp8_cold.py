@@ -55,3 +55,20 @@ def test_first_and_second_run_of_changing_sizes_agree(ops, dtype):
         first, second = (ops.gemm_fp8_tn(*ops_ab[0], *ops_ab[1], out_dtype=dtype) for _ in range(2))
         wrong += (first != second).any()
     assert wrong.item() == 0 and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("M,K,N", [(1000, 2000, 3000), (2048, 1030, 4096), (4096, 640, 8000)])
+def test_both_gradients_from_cold_memory(ops, M, K, N):
+    """The backward's two products, in one launch of CTA pairs where that is quicker: every first run against the next."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    evict = torch.empty(64 << 20, device="cuda")
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(150):
+        x, w, e = (torch.randn(s, generator=g, device="cuda", dtype=torch.bfloat16) for s in ((M, K), (N, K), (M, N)))
+        x, e = (t * torch.exp(2 * torch.randn(M, 1, generator=g, device="cuda")).bfloat16() for t in (x, e))
+        _, saved = ops.fp8_linear_fwd(x, w, True, True, torch.bfloat16)
+        evict.fill_(i)
+        first, second = (ops.fp8_linear_bwd(e, saved, K, torch.float8_e5m2, torch.bfloat16, torch.float32, True, True, True, True) for _ in range(2))
+        for a, b in zip(first, second):
+            wrong += (a != b).any()
+    assert wrong.item() == 0 and ops.device_status() == 0
